@@ -270,7 +270,7 @@ def _plain_balance(s, c):
     B = off.numel() - 1
     row = torch.arange(T, device=l.device)
     of = (row[:, None] >= off[None, 1:].long()).sum(-1)                   # the sequence of a row; B: behind the last
-    live = (l > -math.inf).any(-1) & (of < B)
+    live = (idx >= 0).any(-1) & (of < B)                                  # a token without a choice takes no part
     of = of.clamp_max(B - 1)
     member = ((of[:, None] == torch.arange(B, device=l.device)) & live[:, None]).float()      # [T, B]
     n = member.sum(0)
@@ -391,7 +391,7 @@ def _exact_balance(s, c):
     T, E, K = c["tokens"], c["experts"], c["topk"]
     l = s["logits"].detach().double().requires_grad_(True)
     cuts = [0, T] if s["offsets"] is None else s["offsets"].tolist()
-    some = (l.detach() > -math.inf).any(1)
+    some = (s["idx"] >= 0).any(1)
     terms = []
     for lo, hi in zip(cuts, cuts[1:]):
         rows = torch.arange(lo, hi, device=l.device)[some[lo:hi]]
