@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <chrono>
+#include <cmath>
 #include <cstring>
 #include <map>
 
@@ -13,6 +14,8 @@
 #include "ep/api.h"
 #include "ep/ll_api.h"
 #include "gemm/gemm_api.h"
+#include "norm/norm_api.h"
+#include "route/route_api.h"
 
 namespace py = pybind11;
 using namespace b200ep;
@@ -129,6 +132,8 @@ void check_launch(const char* what) { cuda_ok(cudaGetLastError(), what); }
 #include "bindings_copy.inc"
 #include "bindings_ll.inc"
 #include "bindings_gemm.inc"
+#include "bindings_norm.inc"
+#include "bindings_route.inc"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("MAX_RANKS") = kMaxRanks;
@@ -151,4 +156,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_copy(m);
   bind_ll(m);
   bind_gemm(m);
+  bind_norm(m);
+  bind_route(m);
 }

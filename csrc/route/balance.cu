@@ -1,0 +1,275 @@
+// Loss that keeps the choice of experts balanced, and its gradient. Over the n tokens of a sequence that have a choice, with
+// scores s_t (softmax of the logits, or sigmoid), p_t = s_t / (sum of s_t + 1e-20) and K choices a token:
+//   f_e = E / (K n) * (choices of e),   L = coeff * sum_e f_e * (1 / n) sum_t p_te  [+ z_coeff * (1 / n) sum_t logsumexp(l_t)^2]
+// and the mean over the sequences that have such tokens. f is a count and has no gradient:
+//   softmax: dl_te = c p_te (f_e - F_t),  sigmoid: dl_te = c p_te (1 - s_te) (f_e - F_t),  F_t = sum_j f_j p_tj, c = coeff / (n B')
+//   and 2 z_coeff / (n B') * logsumexp * p_te.
+// With the counts known the loss is a sum over tokens of F_t, so that the logits are read once forward and once backward:
+// a launch that counts the choices (whole numbers: any order gives the same), one that sums F_t (in 64 bits, in a fixed
+// order). Bound: memory for many tokens, launches for few.
+#include "route.cuh"
+
+namespace b200ep {
+namespace route {
+
+// The sequence that row t belongs to, -1 for none: the last one that begins at or before it, if it ends behind it.
+__device__ __forceinline__ int sequence_of(const int* off, int B, long long t) {
+  if (off == nullptr) return 0;
+  int lo = 0, hi = B;                                       // off[lo] <= t < off[hi], if at all
+  if (t < (long long)__ldg(off) || t >= (long long)__ldg(off + B)) return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((long long)__ldg(off + mid) <= t) lo = mid; else hi = mid;
+  }
+  return t < (long long)__ldg(off + lo + 1) ? lo : -1;
+}
+
+// Choices and rows with a choice, counted in shared memory for a run of rows of one sequence at a time.
+__global__ void __launch_bounds__(256)
+balance_count_kernel(const BalanceParams p, int rows_per) {
+  __shared__ int s_count[kRouterMaxExperts];
+  __shared__ int s_rows;
+  const int E = p.E, K = p.K;
+  const long long lo = (long long)blockIdx.x * rows_per, hi = min(lo + rows_per, (long long)p.T);
+  for (long long at = lo; at < hi;) {
+    if (p.seq_off != nullptr) {                             // (rows outside all sequences at either end are passed over at once)
+      if (at >= (long long)__ldg(p.seq_off + p.B)) break;
+      if (at < (long long)__ldg(p.seq_off)) { at = (long long)__ldg(p.seq_off); continue; }
+    }
+    const int b = sequence_of(p.seq_off, p.B, at);
+    long long end = hi;
+    if (p.seq_off != nullptr) {
+      if (b >= 0) end = min(end, (long long)__ldg(p.seq_off + b + 1));
+      else end = at + 1;                                    // (outside every sequence: look at the next row)
+    }
+    if (b >= 0) {
+      for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
+      if (threadIdx.x == 0) s_rows = 0;
+      __syncthreads();
+      for (long long t = at + (threadIdx.x >> 5); t < end; t += blockDim.x >> 5) {
+        const int lane = threadIdx.x & 31;
+        const long long i = lane < K ? p.idx[t * K + lane] : -1;
+        const bool ok = i >= 0 && i < E;
+        if (ok) atomicAdd(s_count + (int)i, 1);
+        if (__any_sync(0xffffffffu, ok) && lane == 0) atomicAdd(&s_rows, 1);
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < E; e += blockDim.x)
+        if (s_count[e]) atomicAdd(p.counts + (long long)b * E + e, s_count[e]);
+      if (threadIdx.x == 0 && s_rows) atomicAdd(p.counts + (long long)p.B * E + b, s_rows);
+      __syncthreads();
+    }
+    at = end;
+  }
+}
+
+// 1 / (sequences with a token that has a choice), the same in every thread of the CTA.
+__device__ __forceinline__ float sequence_share(const BalanceParams& p) {
+  if (p.B == 1) return 1.f;
+  __shared__ int s_live;
+  if (threadIdx.x == 0) s_live = 0;
+  __syncthreads();
+  int n = 0;
+  for (int b = threadIdx.x; b < p.B; b += blockDim.x) n += p.counts[(long long)p.B * p.E + b] > 0;
+  if (n) atomicAdd(&s_live, n);
+  __syncthreads();
+  return 1.f / (float)max(1, s_live);
+}
+
+// What a warp holds of the row it looks at.
+template <typename L, int VPL>
+struct Row {
+  float p[VPL];              // share of the scores
+  float s[VPL];              // sigmoid: 1 - score
+  float lse, F;
+  // false: the row takes no part
+  __device__ __forceinline__ bool load(const BalanceParams& a, long long t, const float* f, int lane) {
+    const long long i = lane < a.K ? a.idx[t * a.K + lane] : -1;
+    const L* row = static_cast<const L*>(a.logits) + t * a.ld;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      p[k] = k * 32 + lane < a.E ? logit(row + k * 32 + lane) : -INFINITY;
+      top = nan_max(p[k], top);
+    }
+    if (!__any_sync(0xffffffffu, i >= 0 && i < a.E)) return false;
+    float sum = 0.f;
+    lse = 0.f;
+    if (a.score == SCORE_SOFTMAX) {
+      top = warp_max(top);
+      if (top == -INFINITY) top = 0.f;
+#pragma unroll
+      for (int k = 0; k < VPL; ++k) { p[k] = expf(p[k] - top); sum += p[k]; }
+      sum = warp_sum(sum);
+      if (a.z_coeff != 0.f && !(sum == 0.f)) lse = top + logf(sum);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VPL; ++k) {
+        const float q = expf(-fabsf(p[k])), r = 1.f / (1.f + q), qr = q * r;
+        const bool up = p[k] >= 0.f;
+        s[k] = up ? qr : r;
+        p[k] = p[k] == -INFINITY ? 0.f : (up ? r : qr);
+        if (q != q) p[k] = q;
+        sum += p[k];
+      }
+      sum = warp_sum(sum);
+    }
+    const float inv = 1.f / (sum + kSumEps);
+    F = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) { p[k] *= inv; F = fmaf(f[k], p[k], F); }
+    F = warp_sum(F);
+    return true;
+  }
+};
+
+// Rows of a warp, a run of neighbours; f of the sequence that they are in is kept in registers.
+template <int VPL>
+struct Walk {
+  int b = -1;
+  float f[VPL], share = 0.f;
+  __device__ __forceinline__ bool to(const BalanceParams& a, long long t, float per_sequence, int lane) {
+    const int now = sequence_of(a.seq_off, a.B, t);
+    if (now < 0) return false;
+    if (now == b) return true;
+    b = now;
+    const int n = max(1, a.counts[(long long)a.B * a.E + b]);
+    const float unit = (float)a.E / ((float)a.K * (float)n);
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) f[k] = k * 32 + lane < a.E ? (float)a.counts[(long long)b * a.E + k * 32 + lane] * unit : 0.f;
+    share = per_sequence / (float)n;
+    return true;
+  }
+};
+
+constexpr int kBalanceWarps = 8;
+
+template <typename L, int VPL>
+__global__ void __launch_bounds__(kBalanceWarps * 32)
+balance_loss_kernel(const BalanceParams p, int rows_per_warp) {
+  __shared__ double s_part[kBalanceWarps];
+  __shared__ bool s_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float per_sequence = sequence_share(p);
+  const long long lo = ((long long)blockIdx.x * kBalanceWarps + warp) * rows_per_warp, hi = min(lo + rows_per_warp, (long long)p.T);
+  Walk<VPL> at;
+  Row<L, VPL> row;
+  double mine = 0.0;
+  for (long long t = lo; t < hi; ++t) {
+    if (!at.to(p, t, per_sequence, lane) || !row.load(p, t, at.f, lane)) continue;
+    mine += (double)at.share * ((double)p.coeff * (double)row.F + (double)p.z_coeff * (double)row.lse * (double)row.lse);
+  }
+  if (lane == 0) s_part[warp] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double v = 0.0;
+    for (int k = 0; k < kBalanceWarps; ++k) v += s_part[k];
+    p.part[blockIdx.x] = v;
+    __threadfence();
+    s_last = atomicAdd(p.counts + (long long)p.B * p.E + p.B, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last || warp != 0) return;
+  __threadfence();
+  double v = 0.0;
+  for (int k = lane; k < (int)gridDim.x; k += 32) v += __ldcg(p.part + k);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0) *p.loss = (float)v;
+}
+
+template <typename L, int VPL>
+__global__ void __launch_bounds__(kBalanceWarps * 32)
+balance_bwd_kernel(const BalanceBwdParams a, int rows_per_warp) {
+  const BalanceParams& p = a.f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float per_sequence = sequence_share(p);
+  const float g = *a.dloss;
+  const long long lo = ((long long)blockIdx.x * kBalanceWarps + warp) * rows_per_warp, hi = min(lo + rows_per_warp, (long long)p.T);
+  Walk<VPL> at;
+  Row<L, VPL> row;
+  for (long long t = lo; t < hi; ++t) {
+    L* out = static_cast<L*>(a.dlogits) + t * p.E;
+    const bool in = at.to(p, t, per_sequence, lane) && row.load(p, t, at.f, lane);
+    const float c = g * at.share * p.coeff, z = 2.f * g * at.share * p.z_coeff * (in ? row.lse : 0.f);
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      if (k * 32 + lane >= p.E) continue;
+      float d = 0.f;
+      if (in) {
+        d = c * (at.f[k] - row.F);
+        if (p.score == SCORE_SIGMOID) d *= row.s[k];
+        d = row.p[k] * (d + z);
+      }
+      put(out + k * 32 + lane, d);
+    }
+  }
+}
+
+inline int rows_a_warp(int T) {
+  // four CTAs of 8 warps on each of 148 SMs, each warp a run of neighbouring rows
+  const long long warps = 148LL * 4 * kBalanceWarps;
+  return (int)((T + warps - 1) / warps) < 1 ? 1 : (int)((T + warps - 1) / warps);
+}
+inline int ctas(int T) {
+  const long long per = (long long)rows_a_warp(T) * kBalanceWarps;
+  return (int)((T + per - 1) / per);
+}
+
+template <typename L, int VPL>
+int forward_sized(const BalanceParams& p, cudaStream_t st) {
+  balance_loss_kernel<L, VPL><<<balance_ctas(p), kBalanceWarps * 32, 0, st>>>(p, rows_a_warp(p.T));
+  return 0;
+}
+template <typename L, int VPL>
+int backward_sized(const BalanceBwdParams& a, cudaStream_t st) {
+  balance_bwd_kernel<L, VPL><<<balance_ctas(a.f), kBalanceWarps * 32, 0, st>>>(a, rows_a_warp(a.f.T));
+  return 0;
+}
+
+#define B200EP_BY_SIZE(E, CALL)              \
+  (E) <= 64 ? CALL(2) : (E) <= 128 ? CALL(4) : (E) <= 256 ? CALL(8) : (E) <= 512 ? CALL(16) : CALL(32)
+
+template <typename L>
+int forward(const BalanceParams& p, cudaStream_t st) {
+#define B200EP_CALL(V) forward_sized<L, V>(p, st)
+  return B200EP_BY_SIZE(p.E, B200EP_CALL);
+#undef B200EP_CALL
+}
+template <typename L>
+int backward(const BalanceBwdParams& a, cudaStream_t st) {
+#define B200EP_CALL(V) backward_sized<L, V>(a, st)
+  return B200EP_BY_SIZE(a.f.E, B200EP_CALL);
+#undef B200EP_CALL
+}
+
+bool fits(const BalanceParams& p) {
+  return p.T >= 0 && p.E >= 1 && p.E <= kRouterMaxExperts && p.K >= 1 && p.K <= kRouteMaxTopk && p.B >= 1 && (p.seq_off != nullptr || p.B == 1) &&
+         (p.z_coeff == 0.f || p.score == SCORE_SOFTMAX);
+}
+
+}  // namespace route
+
+long long balance_words(const BalanceParams& p) { return (long long)p.B * p.E + p.B + 1; }
+int balance_ctas(const BalanceParams& p) { return route::ctas(p.T); }
+
+int launch_balance(const BalanceParams& p, cudaStream_t st) {
+  if (!route::fits(p)) return 1;
+  if (p.T == 0) return cudaMemsetAsync(p.loss, 0, sizeof(float), st) == cudaSuccess ? 0 : 2;
+  if (cudaMemsetAsync(p.counts, 0, (size_t)balance_words(p) * sizeof(int), st) != cudaSuccess) return 2;
+  const int rows_per = (p.T + 295) / 296 < 8 ? 8 : (p.T + 295) / 296;
+  route::balance_count_kernel<<<(p.T + rows_per - 1) / rows_per, 256, 0, st>>>(p, rows_per);
+  if (p.type == ELEM_BF16) return route::forward<__nv_bfloat16>(p, st);
+  if (p.type == ELEM_F16) return route::forward<__half>(p, st);
+  return route::forward<float>(p, st);
+}
+
+int launch_balance_bwd(const BalanceBwdParams& a, cudaStream_t st) {
+  if (!route::fits(a.f)) return 1;
+  if (a.f.T == 0) return 0;
+  if (a.f.type == ELEM_BF16) return route::backward<__nv_bfloat16>(a, st);
+  if (a.f.type == ELEM_F16) return route::backward<__half>(a, st);
+  return route::backward<float>(a, st);
+}
+
+}  // namespace b200ep

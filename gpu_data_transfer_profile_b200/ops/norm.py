@@ -1,0 +1,34 @@
+"""Root-mean-square norm in front of a block, with the residual's addition (csrc/norm).
+
+h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight  over the last dimension, in f32; h and y are rounded once, where
+they are stored (y is that of the sum before its rounding). Rows are bf16, f16 or f32, of 1 to 32768 elements, any number of
+leading dimensions; weights are of the rows' type or f32 (others are taken to f32 first). Two-dimensional inputs may have
+rows further apart than their length; other strides are copied.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+
+from .. import _ext
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
+             eps: float = 1e-6) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """y, or (y, h) with a residual (shape and type of x): h is the residual of the next block.
+
+    Differentiable once in x, residual and weight; the weight's gradient is summed in a fixed order. No forward-mode
+    derivatives, no function transforms (refused)."""
+    y, h = _ext.load().rms_norm(x, weight, residual, eps)
+    return y if residual is None else (y, h)
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 keep: bool = False) -> Tuple[Tuple[torch.Tensor, torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """-> ((q e4m3 [..., H], scales f32 [..., H/128]), y, h): what `Buffer.dispatch` takes in place of rows and
+    `ops.gemm.grouped_gemm_fp8` multiplies; scale = max(amax, 1e-4) / 448 of 128 channels of y, as in the cast of an fp8
+    dispatch, here of y before its rounding. y in the type of x if `keep` (for a router beside the experts), else None; h is
+    None without a residual. H is a multiple of 128. For inference: refuses inputs that require a gradient."""
+    q, scales, y, h = _ext.load().rms_norm_fp8(x, weight, residual, eps, keep)
+    return (q, scales), y, h
