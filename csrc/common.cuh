@@ -192,6 +192,13 @@ inline cudaError_t launch_ordered(void (*kern)(KArgs...), dim3 grid, dim3 block,
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
+// Multiprocessors of the current device.
+inline int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return n;
+}
+
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 31; }
 
 // "Last block done" bookkeeping: every block calls this once after its work; exactly one

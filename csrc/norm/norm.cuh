@@ -133,11 +133,5 @@ inline int align_period(long long ld_bytes) {
   return p;
 }
 
-inline int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return n;
-}
-
 }  // namespace norm
 }  // namespace b200ep

@@ -21,6 +21,11 @@ struct Key32 {
     const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
     return v == -INFINITY ? 0u : k;
   }
+  // The value of a key, not a number for the largest ones; -inf for 0.
+  static __device__ __forceinline__ float value(uint32_t k) {
+    if (k == 0u) return -INFINITY;
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+  }
 };
 struct Key64 {
   using V = double;
@@ -40,19 +45,9 @@ __device__ __forceinline__ unsigned long long warp_best(unsigned long long k) {
   return ((unsigned long long)top << 32) | lo;
 }
 
-// Groups that stay, one bit each. s_v: the warp's choice values [E] in shared memory. Lane g looks at group g.
+// How many groups go before this lane's: higher values (not a number above all), the lower index among equals.
 template <typename V>
-__device__ __forceinline__ uint32_t groups_kept(const V* s_v, int groups, int size, int keep, int best, int lane) {
-  V a = -INFINITY, b = -INFINITY;                           // the two highest
-  if (lane < groups) {
-    for (int j = 0; j < size; ++j) {
-      const V v = s_v[lane * size + j];
-      if (v > a || v != v) { b = a; a = v; }
-      else if (v > b) b = v;
-    }
-  }
-  V mine = best == 2 && b > (V)-INFINITY ? a + b : a;
-  if (a != a || b != b) mine = a + b;
+__device__ __forceinline__ int groups_ahead(V mine, int groups, int lane) {
   const bool none = mine != mine;
   int ahead = 0;
   for (int g = 0; g < groups; ++g) {
@@ -61,79 +56,96 @@ __device__ __forceinline__ uint32_t groups_kept(const V* s_v, int groups, int si
     const bool equal = o == mine || (o_none && none);
     ahead += (!none && (o_none || o > mine)) || (equal && g < lane);
   }
-  return __ballot_sync(0xffffffffu, lane < groups && ahead < keep);
+  return ahead;
 }
 
+// How the experts lie over the lanes: `lanes` neighbouring lanes (a power of two) have a group, each a run of `chunk` of its
+// experts, so that a lane's values are all of one group and rise in index from lane to lane. Without groups, or where all
+// of them stay, the experts are one group.
+struct Groups {
+  int count, size;           // groups that are told apart, experts of each
+  int lanes, chunk;
+  uint32_t mask;             // of the bits that tell groups apart
+  bool vec;                  // every lane's run is whole and its loads of 4 values are aligned
+  // choose_exactly's: the groups again (for 17 to 31 groups of more than 32, which leave a lane too many values, they are
+  // told apart there alone, for every token), and e / size == e * magic >> 20 for e, size <= 1024: the error
+  // e * (magic * size - 2^20) stays below 2^20
+  bool exact;
+  int told, magic;
+};
+__device__ __forceinline__ int group_of(const Groups& g, int e) { return (int)((uint32_t)e * (uint32_t)g.magic >> 20); }
+
+// ---- the choice as it is defined: every value compared, in 64 bits where they are computed -------------------------------
+// Lane k's choice, -1 for none. Called where the quick way below cannot tell neighbours apart, for few tokens.
 template <typename L, int VPL, typename KEY>
-__global__ void __launch_bounds__(256)
-route_kernel(const RouteParams p, int size_magic) {
+__device__ __noinline__ int choose_exactly(const RouteParams& p, const L* row, const Groups& gr) {
   using V = typename KEY::V;
   using K = decltype(KEY::of(V(0)));
-  extern __shared__ __align__(16) char s_raw[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E;
-  const long long t = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
-  if (t >= p.T) return;
-  const L* row = static_cast<const L*>(p.logits) + t * p.ld;
-  float l[VPL];
-  float top = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    l[i] = i * 32 + lane < E ? logit(row + i * 32 + lane) : -INFINITY;
-    top = nan_max(l[i], top);
-  }
-  const bool soft = p.score == SCORE_SOFTMAX;
-  top = warp_max(top);
-  if (soft) {
-    if (top == -INFINITY) top = 0.f;                        // no expert is available: all scores are 0
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) sum += expf(l[i] - top);
-    sum = warp_sum(sum);
-  }
-  // the values that are compared
+  const int lane = threadIdx.x & 31, E = p.E;
   K key[VPL];
+  V v[VPL];
   if constexpr (sizeof(V) == 8) {
-    double total = 0.0;
-    V v[VPL];
+    V top = -INFINITY, total = 0.0;
+    const bool soft = p.score == SCORE_SOFTMAX;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      v[i] = i * 32 + lane < E ? (V)logit(row + i * 32 + lane) : (V)-INFINITY;
+      top = v[i] > top || v[i] != v[i] ? v[i] : top;
+    }
     if (soft) {
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) total += v[i] = exp((double)l[i] - (double)top);
+      for (int o = 16; o > 0; o >>= 1) {
+        const V w = __shfl_xor_sync(0xffffffffu, top, o);
+        top = w > top || w != w ? w : top;
+      }
+      if (top == -INFINITY) top = 0.0;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) total += exp(v[i] - top);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int e = i * 32 + lane;
-      v[i] = soft ? v[i] / total : 1.0 / (1.0 + exp(-(double)l[i]));
-      if (p.bias != nullptr && e < E) v[i] += (double)__ldg(p.bias + e);
-      if (l[i] == -INFINITY) v[i] = -INFINITY;
-      key[i] = KEY::of(v[i]);
-    }
-    if (p.groups > 1) {
-      V* s_v = reinterpret_cast<V*>(s_raw) + (size_t)warp * E;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (i * 32 + lane < E) s_v[i * 32 + lane] = v[i];
+      const bool absent = v[i] == -INFINITY;
+      v[i] = soft ? exp(v[i] - top) / total : 1.0 / (1.0 + exp(-v[i]));
+      if (p.bias != nullptr && e < E) v[i] += (V)__ldg(p.bias + e);
+      if (absent) v[i] = -INFINITY;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) key[i] = KEY::of(l[i]);
-    if (p.groups > 1) {
-      V* s_v = reinterpret_cast<V*>(s_raw) + (size_t)warp * E;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (i * 32 + lane < E) s_v[i * 32 + lane] = l[i];
-    }
+    for (int i = 0; i < VPL; ++i) v[i] = i * 32 + lane < E ? logit(row + i * 32 + lane) : -INFINITY;
   }
-  if (p.groups > 1) {
-    __syncwarp();
-    const uint32_t kept = groups_kept(reinterpret_cast<const V*>(s_raw) + (size_t)warp * E, p.groups, E / p.groups, p.topk_groups, p.group_best, lane);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const uint32_t g = (uint32_t)(i * 32 + lane) * (uint32_t)size_magic >> 20;      // (i * 32 + lane) / size
-      if (i * 32 + lane < E && !(kept >> g & 1)) key[i] = 0;
+  for (int i = 0; i < VPL; ++i) key[i] = KEY::of(v[i]);
+  if (gr.told > 1) {
+    // group after group: the lanes' two highest, then the warp's (a sum of two is the same whichever way it is found)
+    V mine = -INFINITY;                                     // lane g: the value of group g
+    for (int g = 0; g < gr.told; ++g) {
+      V a = -INFINITY, b = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        if (group_of(gr, i * 32 + lane) != g || i * 32 + lane >= E) continue;
+        if (v[i] > a || v[i] != v[i]) { b = a; a = v[i]; }
+        else if (v[i] > b) b = v[i];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const V c = __shfl_xor_sync(0xffffffffu, a, o), d = __shfl_xor_sync(0xffffffffu, b, o);
+        const V low = a != a || c != c ? c + a : (c > a ? a : c);        // (not a number stays in the sum)
+        a = a != a || c != c ? c + a : (c > a ? c : a);
+        b = b > d ? b : d;
+        b = low > b || low != low ? low : b;
+      }
+      const V value = a != a ? a : (p.group_best == 2 && b > (V)-INFINITY ? a + b : a);
+      if (lane == g) mine = value;
     }
+    const int ahead = groups_ahead(mine, gr.told, lane);
+    const uint32_t kept = __ballot_sync(0xffffffffu, lane < gr.told && ahead < p.topk_groups);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (!(kept >> (group_of(gr, i * 32 + lane) & 31) & 1)) key[i] = 0;
   }
-  float mine_l = 0.f;                                       // lane k: the logit of choice k
   int mine_e = -1;
   for (int k = 0; k < p.K; ++k) {
     K best = 0;
@@ -144,22 +156,372 @@ route_kernel(const RouteParams p, int size_magic) {
     const K high = warp_best(best);
     if (high == 0) break;                                   // nothing is left
     const uint32_t e = __reduce_min_sync(0xffffffffu, best == high ? (uint32_t)(at * 32 + lane) : 0xffffffffu);
-    float le = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if ((int)e == i * 32 + lane) { le = l[i]; key[i] = 0; }
-    le = __shfl_sync(0xffffffffu, le, e & 31);
-    if (lane == k) { mine_l = le; mine_e = (int)e; }
+      if ((int)e == i * 32 + lane) key[i] = 0;
+    if (lane == k) mine_e = (int)e;
   }
-  float s = 0.f;
-  if (mine_e >= 0) s = soft ? expf(mine_l - top) / sum : 1.f / (1.f + expf(-mine_l));
-  const float chosen = warp_sum(s);
-  if (lane < p.K) {
-    p.idx[t * p.K + lane] = mine_e;
-    p.w[t * p.K + lane] = mine_e < 0 ? 0.f : (p.renorm ? s / (chosen + kSumEps) : s) * p.scale;
-    if (p.aux != nullptr && !soft) p.aux[t * p.K + lane] = mine_l;
+  return mine_e;
+}
+
+// ---- the quick way -------------------------------------------------------------------------------------------------------
+// Keys of 32 bits whose low bits say which of the lane's values they are, sorted in each lane, so that a choice is one warp
+// maximum of the lanes' first keys. How far a key's value may be from the one it stands for is known; where neighbours
+// among the choices, and the values after the last one, lie closer than that, they are compared again as they are defined
+// (settle: one lane each), so are groups that close to the last one that stays (settle_groups). More than 32 such values
+// are left to choose_exactly. 256 sigmoid scores with a bias: about one token in 200 is settled, one in 1000 for its groups.
+//   kLogit16: 16-bit logits rank by themselves; the low half of a key is the expert, the lowest highest: always told apart
+//   kLogit32: 32-bit logits rank by themselves, but for the low bits that the place in the lane takes
+//   kComputed: scores and a bias in 32 bits, also but for those low bits
+enum Mode : int { kLogit16 = 0, kLogit32 = 1, kComputed = 2 };
+
+// A float's bits in the order of its values (-0 just below 0). Keys up to kAbsent, that of -inf, stand for nothing.
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+constexpr uint32_t kAbsent = 0x007fffffu;
+
+template <int N> constexpr int kLog2 = 1 + kLog2<(N + 1) / 2>;
+template <> constexpr int kLog2<1> = 0;
+
+// Descending, by Batcher's odd-even merges.
+template <int N>
+__device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const uint32_t a = k[i + j], b = k[i + j + q];
+            k[i + j] = max(a, b);
+            k[i + j + q] = min(a, b);
+          }
+}
+
+// 1 / y, off by little more than half a unit in the last place: the hardware's approximation and one step of Newton's
+// iteration; without the branches of a division.
+__device__ __forceinline__ float reciprocal(float y) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return y < INFINITY ? fmaf(r, fmaf(-y, r, 1.f), r) : r;
+}
+// 1 / (1 + exp(-x)) from the hardware's approximations: off by less than 2^-21.
+__device__ __forceinline__ float quick_sigmoid(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-x)));
+  return r;
+}
+
+// The values that are compared, as they are defined: of 64 bits where they are computed.
+template <int MODE>
+struct Defined {
+  using V = typename std::conditional<MODE == kComputed, double, float>::type;
+  using KEY = typename std::conditional<MODE == kComputed, Key64, Key32>::type;
+  V top = 0, total = 0;
+  // by the whole warp
+  template <typename L>
+  __device__ __forceinline__ void row(const RouteParams& p, const L* row) {
+    if (MODE != kComputed || p.score != SCORE_SOFTMAX) return;
+    const int lane = threadIdx.x & 31;
+    top = -INFINITY;
+    for (int j = lane; j < p.E; j += 32) {
+      const V l = (V)logit(row + j);
+      top = l > top || l != l ? l : top;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const V w = __shfl_xor_sync(0xffffffffu, top, o);
+      top = w > top || w != w ? w : top;
+    }
+    for (int j = lane; j < p.E; j += 32) total += exp((V)logit(row + j) - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
-  if (p.aux != nullptr && soft && !p.renorm && lane < 2) p.aux[t * 2 + lane] = lane == 0 ? top : (sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+  template <typename L>
+  __device__ __forceinline__ V of(const RouteParams& p, const L* row, int e) const {
+    V v = (V)logit(row + e);
+    if constexpr (MODE == kComputed) {
+      if (v == (V)-INFINITY) return v;
+      v = p.score == SCORE_SOFTMAX ? exp(v - top) / total : 1.0 / (1.0 + exp(-v));
+      if (p.bias != nullptr) v += (V)__ldg(p.bias + e);
+    }
+    return v;
+  }
+};
+
+// The n candidates, one a lane (e), in their defined order: the expert of lane k's choice.
+template <typename L, int MODE>
+__device__ __noinline__ int settle(const RouteParams& p, const L* row, int e, int n) {
+  Defined<MODE> d;
+  d.row(p, row);
+  const int lane = threadIdx.x & 31;
+  const auto key = Defined<MODE>::KEY::of(lane < n ? d.of(p, row, e) : 0);
+  int ahead = 0;
+  for (int j = 0; j < n; ++j) {
+    const auto o = __shfl_sync(0xffffffffu, key, j);
+    const int oe = __shfl_sync(0xffffffffu, e, j);
+    ahead += o > key || (o == key && oe < e);
+  }
+  int mine = -1;
+  for (int j = 0; j < n; ++j) {
+    const int oe = __shfl_sync(0xffffffffu, e, j), place = __shfl_sync(0xffffffffu, ahead, j);
+    if (place == lane) mine = oe;
+  }
+  return mine;
+}
+
+// Of the groups in `among`, one bit each, those `keep` that have the highest values as they are defined.
+template <typename L, int MODE>
+__device__ __noinline__ uint32_t settle_groups(const RouteParams& p, const L* row, int size, uint32_t among, int keep) {
+  using V = typename Defined<MODE>::V;
+  Defined<MODE> d;
+  d.row(p, row);
+  const int lane = threadIdx.x & 31;
+  V mine = -INFINITY;                                       // lane g: the value of group g
+  for (uint32_t left = among; left != 0u; left &= left - 1) {
+    const int g = __ffs(left) - 1;
+    V a = -INFINITY, b = -INFINITY;                         // the two highest; not a number above all
+    for (int j = lane; j < size; j += 32) {
+      const V v = d.of(p, row, g * size + j);
+      if (v > a || v != v) { b = a; a = v; }
+      else if (v > b) b = v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const V c = __shfl_xor_sync(0xffffffffu, a, o), f = __shfl_xor_sync(0xffffffffu, b, o);
+      const bool none = a != a || c != c;
+      const V low = c > a ? a : c;
+      a = none ? a + c : (c > a ? c : a);
+      b = b > f ? b : f;
+      b = !none && low > b ? low : b;
+    }
+    if (lane == g) mine = a != a ? a : (p.group_best == 2 && b > (V)-INFINITY ? a + b : a);
+  }
+  const bool in = among >> lane & 1;
+  int ahead = 0;
+  for (uint32_t left = among; left != 0u; left &= left - 1) {
+    const int g = __ffs(left) - 1;
+    const V o = __shfl_sync(0xffffffffu, mine, g);
+    ahead += (mine == mine && (o != o || o > mine)) || ((o == mine || (o != o && mine != mine)) && g < lane);
+  }
+  return __ballot_sync(0xffffffffu, in && ahead < keep);
+}
+
+// The 16 bits of a 16-bit logit in the order of its values, in the upper half.
+__device__ __forceinline__ uint32_t order16(float v, const __nv_bfloat16*) { return order_of(v) & 0xffff0000u; }
+__device__ __forceinline__ uint32_t order16(float v, const __half*) {
+  if (v == -INFINITY) return 0u;
+  const uint32_t u = (uint32_t)__half_as_ushort(__float2half_rn(v)) << 16;
+  return (u ^ ((uint32_t)((int)u >> 31) | 0x80000000u)) & 0xffff0000u;
+}
+__device__ __forceinline__ uint32_t order16(float v, const float*) { return 0u; }      // (has no such mode)
+
+template <typename L> struct Four;           // four logits in one load
+template <> struct Four<float> {
+  static __device__ __forceinline__ void get(const float* p, float* f) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  }
+};
+template <> struct Four<__nv_bfloat16> {
+  static __device__ __forceinline__ void get(const __nv_bfloat16* p, float* f) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+};
+template <> struct Four<__half> {
+  static __device__ __forceinline__ void get(const __half* p, float* f) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+  }
+};
+
+template <typename L, int VPL, int MODE>
+__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2)
+route_kernel(const __grid_constant__ RouteParams p, const __grid_constant__ Groups gr) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const bool soft = p.score == SCORE_SOFTMAX;
+  constexpr int LOW = MODE == kLogit16 ? 0 : kLog2<VPL>;    // bits of a key that say where it came from
+  constexpr uint32_t MASK = (1u << LOW) - 1;
+  const int group = lane / gr.lanes, sub = lane & (gr.lanes - 1);
+  const int e0 = group * gr.size + sub * gr.chunk;          // the lane's first expert, and how many it has
+  const int mine_n = group < gr.count ? max(0, min(gr.chunk, gr.size - sub * gr.chunk)) : 0;
+  float bias[VPL], most_bias = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    bias[i] = MODE == kComputed && p.bias != nullptr && i < mine_n ? __ldg(p.bias + e0 + i) : 0.f;
+    if (fabsf(bias[i]) < INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
+  }
+  if (MODE == kComputed) most_bias = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_bias)));
+  for (long long t = (long long)blockIdx.x * warps + warp; t < p.T; t += (long long)gridDim.x * warps) {
+    const L* row = static_cast<const L*>(p.logits) + t * p.ld;
+    float l[VPL];
+    float top = 0.f, sum = 0.f;
+    bool loaded = false;
+    if constexpr (VPL % 4 == 0) {
+      if (gr.vec) {
+#pragma unroll
+        for (int i = 0; i < VPL; i += 4) {
+          l[i] = l[i + 1] = l[i + 2] = l[i + 3] = -INFINITY;
+          if (i < mine_n) Four<L>::get(row + e0 + i, l + i);
+        }
+        loaded = true;
+      }
+    }
+    if (!loaded) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) l[i] = i < mine_n ? logit(row + e0 + i) : -INFINITY;
+    }
+    if (soft) {
+      top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) top = nan_max(l[i], top);
+      top = warp_max(top);
+      if (top == -INFINITY) top = 0.f;                      // no expert is available: all scores are 0
+    }
+    uint32_t key[VPL];
+    float margin = 0.f;                                     // how far a key's value may be from the one it stands for
+    bool odd = false;                                       // not a number among logits that are compared as they are
+    if constexpr (MODE == kComputed) {
+      float s[VPL], unit = 1.f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) s[i] = soft ? __expf(l[i] - top) : quick_sigmoid(l[i]);
+      if (soft) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) sum += s[i];
+        sum = warp_sum(sum);
+        unit = reciprocal(sum);
+      }
+      // A sigmoid is off by 2^-21 of at most 1. A softmax score p has its exponential off by 2 units in the last place and, for
+      // the distance d to the maximum, by 2 d 2^-24 of itself, which p = e^-d / sum makes less than 2^-24 of the largest, 1 / sum;
+      // and a sum of VPL + 5 roundings and those of its terms: 2^-18 of the largest covers all. The sum with the bias is
+      // rounded once, its key has LOW bits of its own.
+      margin = (soft ? 0x1p-18f * unit : 0x1p-21f) + (float)(1 + (1 << LOW)) * 0x1p-23f * (unit + most_bias);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const float c = l[i] == -INFINITY ? -INFINITY : fmaf(s[i], unit, bias[i]);
+        key[i] = (order_of(c) & ~MASK) | (uint32_t)(VPL - 1 - i);        // (a sum that is not a number has the highest)
+      }
+    } else {
+      if (soft) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) sum += __expf(l[i] - top);
+        sum = warp_sum(sum);
+      }
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        odd = odd || l[i] != l[i];
+        if constexpr (MODE == kLogit16) {
+          key[i] = order16(l[i] + 0.f, row);
+          key[i] |= key[i] > kAbsent ? (uint32_t)(0xffff - (e0 + i)) : 0u;
+        } else {
+          key[i] = (order_of(l[i]) & ~MASK) | (uint32_t)(VPL - 1 - i);
+        }
+      }
+    }
+    // whether two values, the first with the higher key, are in this order for certain
+    const auto apart = [&](uint32_t high, uint32_t low) {
+      if (MODE == kLogit16 || low <= kAbsent) return true;
+      if (MODE == kLogit32) return (high & ~MASK) > (low & ~MASK) && !(low >= (0x7fffffffu & ~MASK) && high <= (0x80000000u | MASK));      // (-0 is 0)
+      return Key32::value(high) - Key32::value(low) > 2.f * margin;
+    };
+    sort_keys(key);
+    bool exact = gr.exact || (MODE != kComputed && __any_sync(0xffffffffu, odd));
+    if (gr.count > 1) {
+      // the group's two highest, in all of its lanes
+      uint32_t a = key[0], b = key[1];
+      for (int o = gr.lanes >> 1; o > 0; o >>= 1) {
+        const uint32_t c = __shfl_xor_sync(0xffffffffu, a, o), d = __shfl_xor_sync(0xffffffffu, b, o);
+        b = max(min(a, c), max(b, d));
+        a = max(a, c);
+      }
+      // its value as a key that is its own: the low bits say which group (a logit of 16 bits has them already), lowest first
+      if (MODE == kComputed && p.group_best == 2 && b > kAbsent) a = order_of(Key32::value(a) + Key32::value(b));
+      if (MODE != kLogit16 && a > kAbsent) a = (a & ~gr.mask) | (gr.mask - (uint32_t)group);
+      uint32_t left = a, last = 0u;
+      for (int k = 0; k < p.topk_groups; ++k) {
+        last = __reduce_max_sync(0xffffffffu, left);
+        if (left == last) left = 0u;
+      }
+      bool kept = left == 0u;
+      if constexpr (MODE != kLogit16) {
+        // (two values of either side, their sums' rounding and the keys' own bits; -0 and 0 lie within a step of 2^-149)
+        const uint32_t next = __reduce_max_sync(0xffffffffu, left);
+        const uint32_t low = gr.mask | MASK;
+        const float about = MODE == kComputed ? 4.f * margin + (float)(2 + 2 * low) * 0x1p-23f * fabsf(Key32::value(last)) : 0.f;
+        const bool close = next > kAbsent && (MODE == kLogit32 ? (last & ~low) == (next & ~low) || (next >= (0x7fffffffu & ~low) && last <= (0x80000000u | low))
+                                                              : !(Key32::value(last) - Key32::value(next) > about));
+        if (close && !exact) {
+          // those near the last one that stays are looked at again, the others are in or out
+          bool in, near;
+          if (MODE == kLogit32) {
+            const uint32_t zero = 0x80000000u & ~low, at = (last & ~low) == (0x7fffffffu & ~low) ? zero : last & ~low;
+            const uint32_t me = (a & ~low) == (0x7fffffffu & ~low) ? zero : a & ~low;
+            near = a > kAbsent && me == at;
+            in = a > kAbsent && me > at;
+          } else {
+            const float off = Key32::value(a) - Key32::value(last);
+            near = a > kAbsent && !(fabsf(off) > about);
+            in = a > kAbsent && off > about;
+          }
+          const uint32_t first = __ballot_sync(0xffffffffu, (lane & (gr.lanes - 1)) == 0 && group < gr.count);
+          const uint32_t in_lanes = __ballot_sync(0xffffffffu, in) & first, near_lanes = __ballot_sync(0xffffffffu, near) & first;
+          uint32_t among = 0u;
+          for (uint32_t m = near_lanes; m != 0u; m &= m - 1) among |= 1u << ((__ffs(m) - 1) / gr.lanes);
+          const uint32_t stay = settle_groups<L, MODE>(p, row, gr.size, among, p.topk_groups - __popc(in_lanes));
+          kept = in || (near && (stay >> group & 1));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) key[i] = kept ? key[i] : 0u;
+    }
+    // lane k keeps choice k; behind the last one, the values that may change places with it
+    uint32_t mine = 0u, high = 0u;
+    int from = 0, n = 0;
+    for (; n < 32; ++n) {
+      const uint32_t before = high;
+      high = __reduce_max_sync(0xffffffffu, key[0]);
+      if (high <= kAbsent || (n >= p.K && apart(before, high))) break;
+      const int at = __ffs(__ballot_sync(0xffffffffu, key[0] == high)) - 1;
+      if (lane == n) { mine = high; from = at; }
+      if (lane == at) {
+#pragma unroll
+        for (int i = 0; i + 1 < VPL; ++i) key[i] = key[i + 1];
+        key[VPL - 1] = 0u;
+      }
+    }
+    int mine_e = __shfl_sync(0xffffffffu, e0, from) + VPL - 1 - (int)(mine & MASK);
+    if (MODE == kLogit16) mine_e = 0xffff - (int)(mine & 0xffffu);
+    if (lane >= n) mine_e = -1;
+    if constexpr (MODE != kLogit16) {
+      const uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
+      const bool doubt = n > p.K || __any_sync(0xffffffffu, lane + 1 < n && !apart(mine, after));
+      // (32 of them, and the next may be as close)
+      exact = exact || (n == 32 && !apart(__shfl_sync(0xffffffffu, mine, 31), __reduce_max_sync(0xffffffffu, key[0])));
+      if (doubt && !exact) mine_e = settle<L, MODE>(p, row, mine_e, n);
+    }
+    if (exact) mine_e = choose_exactly<L, VPL, typename Defined<MODE>::KEY>(p, row, gr);
+    if (lane >= p.K) mine_e = -1;
+    float mine_l = 0.f, s = 0.f;
+    if (mine_e >= 0) {
+      mine_l = logit(row + mine_e);
+      s = soft ? expf(mine_l - top) * reciprocal(sum) : reciprocal(1.f + expf(-mine_l));
+    }
+    const float chosen = warp_sum(s);
+    if (lane < p.K) {
+      p.idx[t * p.K + lane] = mine_e;
+      p.w[t * p.K + lane] = mine_e < 0 ? 0.f : (p.renorm ? s * reciprocal(chosen + kSumEps) : s) * p.scale;
+      if (p.aux != nullptr && !soft) p.aux[t * p.K + lane] = mine_l;
+    }
+    if (p.aux != nullptr && soft && !p.renorm && lane < 2) p.aux[t * 2 + lane] = lane == 0 ? top : (sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+  }
 }
 
 // Gradient of the logits, a warp per token. With g the weights' gradient times `scale`:
@@ -212,30 +574,49 @@ route_bwd_kernel(const RouteBwdParams p) {
   if (e >= 0) put(out + e, d);
 }
 
-template <typename L, int VPL, typename KEY>
-int launch_sized(const RouteParams& p, cudaStream_t st) {
+template <typename L, int VPL, int MODE>
+int launch_sized(const RouteParams& p, const Groups& g, cudaStream_t st) {
   const int warps = p.T < 1184 ? 1 : 8;
-  const int size = p.E / p.groups;
-  // e / size == e * magic >> 20 for e, size <= 1024: the error e * (magic * size - 2^20) stays below 2^20
-  const int magic = ((1 << 20) + size - 1) / size;
-  const size_t smem = p.groups > 1 ? (size_t)warps * p.E * sizeof(typename KEY::V) : 0;
-  const auto kern = route_kernel<L, VPL, KEY>;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 2;
-  kern<<<(int)(((long long)p.T + warps - 1) / warps), warps * 32, smem, st>>>(p, magic);
+  const auto kern = route_kernel<L, VPL, MODE>;
+  int fit = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, warps * 32, 0) != cudaSuccess || fit < 1) return 2;
+  const long long need = ((long long)p.T + warps - 1) / warps, most = (long long)fit * sm_count();
+  kern<<<(int)(need < most ? need : most), warps * 32, 0, st>>>(p, g);
   return 0;
 }
-template <typename L, typename KEY>
-int launch_keyed(const RouteParams& p, cudaStream_t st) {
-  if (p.E <= 64) return launch_sized<L, 2, KEY>(p, st);
-  if (p.E <= 128) return launch_sized<L, 4, KEY>(p, st);
-  if (p.E <= 256) return launch_sized<L, 8, KEY>(p, st);
-  if (p.E <= 512) return launch_sized<L, 16, KEY>(p, st);
-  return launch_sized<L, 32, KEY>(p, st);
+template <typename L, int MODE>
+int launch_mode(const RouteParams& p, cudaStream_t st) {
+  Groups g{};
+  g.count = p.topk_groups < p.groups ? p.groups : 1;
+  g.size = p.E / g.count;
+  g.told = g.count;
+  g.magic = ((1 << 20) + g.size - 1) / g.size;
+  const auto lay = [&g] {
+    g.lanes = 32;
+    while (g.lanes * g.count > 32) g.lanes >>= 1;
+    g.chunk = (g.size + g.lanes - 1) / g.lanes;
+  };
+  lay();
+  if (g.chunk > 32) {
+    g.exact = true;
+    g.count = 1;
+    g.size = p.E;
+    lay();
+  }
+  g.mask = 0u;
+  while ((int)g.mask + 1 < g.count) g.mask = 2 * g.mask + 1;
+  g.vec = g.chunk % 4 == 0 && g.size % g.chunk == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(L)) == 0;
+  if (g.chunk <= 2) return launch_sized<L, 2, MODE>(p, g, st);
+  if (g.chunk <= 4) return launch_sized<L, 4, MODE>(p, g, st);
+  if (g.chunk <= 8) return launch_sized<L, 8, MODE>(p, g, st);
+  if (g.chunk <= 16) return launch_sized<L, 16, MODE>(p, g, st);
+  return launch_sized<L, 32, MODE>(p, g, st);
 }
 template <typename L>
 int launch_typed(const RouteParams& p, cudaStream_t st) {
-  const bool computed = p.bias != nullptr || (p.groups > 1 && p.group_best == 2);
-  return computed ? launch_keyed<L, Key64>(p, st) : launch_keyed<L, Key32>(p, st);
+  const bool computed = p.bias != nullptr || (p.topk_groups < p.groups && p.group_best == 2);
+  if (computed) return launch_mode<L, kComputed>(p, st);
+  return launch_mode<L, sizeof(L) == 2 ? kLogit16 : kLogit32>(p, st);
 }
 
 }  // namespace route

@@ -30,7 +30,7 @@ def route(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias: Opti
     weights and has no gradient): of `num_groups` runs of E / num_groups neighbours those `topk_groups` (default: all) stay
     whose `group_best` (1 or 2) best v have the highest sum, and of their experts the topk with the highest v are chosen, in
     descending order; the lower index goes first among equals. v is compared as 64 bits have it, the logits themselves where
-    there is neither a bias nor a sum of two. Weights are the chosen s, over their sum + 1e-20 with `renormalize`, times `scale`.
+    neither a bias nor a sum of two has a part in the choice. Weights are the chosen s, over their sum + 1e-20 with `renormalize`, times `scale`.
 
     An expert whose logit or bias is -inf is not available: where fewer than topk are left, the index is -1 (no expert, to
     every call of this package) and the weight 0, for all choices of a padding row. NaN ranks above everything. topk and

@@ -81,7 +81,8 @@ CASES = [  # T, E, K, score, bias, groups, topk_groups, best
     (90, 96, 1, "sigmoid", True, 32, 1, 2), (90, 96, 3, "softmax", False, 32, 1, 1), (50, 384, 8, "sigmoid", True, 1, 1, 1),
     (40, 1024, 32, "sigmoid", True, 16, 2, 2), (40, 1000, 32, "softmax", False, 1, 1, 1), (40, 1023, 9, "softmax", True, 31, 11, 1),
     (64, 128, 32, "sigmoid", False, 4, 1, 2), (1300, 72, 5, "sigmoid", True, 3, 2, 2), (2500, 512, 8, "softmax", True, 2, 1, 1),
-    (20, 32, 4, "sigmoid", True, 32, 7, 2), (20, 40, 4, "softmax", True, 20, 7, 2), (20, 7, 7, "sigmoid", True, 7, 7, 2),
+    (20, 32, 4, "sigmoid", True, 32, 7, 2), (60, 1020, 9, "softmax", True, 17, 5, 2), (60, 1020, 32, "sigmoid", False, 17, 5, 1),
+    (400, 160, 8, "sigmoid", True, 8, 3, 2), (400, 336, 8, "softmax", True, 7, 3, 2), (20, 40, 4, "softmax", True, 20, 7, 2), (20, 7, 7, "sigmoid", True, 7, 7, 2),
 ]
 
 
@@ -154,6 +155,41 @@ def test_route_of_neighbours_that_32_bits_do_not_tell_apart():
     want = _choose(l.double().cpu().numpy(), 5, "sigmoid", bias.double().cpu().numpy(), 4, 2, 2)
     idx, _ = route(l, 5, score="sigmoid", bias=bias, num_groups=4, topk_groups=2, group_best=2)
     assert torch.equal(idx.cpu(), torch.from_numpy(want))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,topk_groups,best,grid", [(256, 8, 4, 2, 0), (256, 8, 4, 1, 16), (160, 8, 3, 2, 8), (96, 32, 9, 2, 16), (64, 1, 1, 1, 4), (72, 3, 2, 1, 0),
+                                                          (512, 16, 3, 2, 0), (40, 4, 1, 2, 4)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_of_many_tokens(E, groups, topk_groups, best, grid, biased, score):
+    """Tokens by the ten thousand, among them many with equal logits (on a grid) and values a few 32-bit steps apart."""
+    from gpu_data_transfer_profile_b200.ops.router import route
+    T, K = 20000, 7
+    g = torch.Generator(device="cuda").manual_seed(E + grid)
+    l = torch.randn(T, E, generator=g, device="cuda")
+    if grid:
+        l = (l * grid).round() / grid
+    bias = (torch.rand(E, generator=g, device="cuda") - 0.5) * 0.3
+    if grid:
+        bias = (bias * 16).round() / 16
+    close = torch.rand(T, E, generator=g, device="cuda") < 0.2    # a value and its neighbour on the next place but for some steps
+    close[:, ::2] = False
+    l = torch.where(close, torch.roll(l, 1, 1) * (1 + torch.randint(-3, 4, (T, E), generator=g, device="cuda") * 2.0 ** -24), l)
+    w = l.double()
+    s = torch.sigmoid(w) if score == "sigmoid" else torch.softmax(w, 1)
+    computed = biased or (groups > 1 and best == 2)
+    v = (s if computed else w) + (bias.double() if biased else 0)
+    if groups > 1:
+        value = v.view(T, groups, -1).topk(best, -1).values.sum(-1)
+        order = torch.sort(value, dim=1, descending=True, stable=True).indices[:, :topk_groups]
+        kept = torch.zeros(T, groups, dtype=torch.bool, device="cuda").scatter_(1, order, True)
+        v = torch.where(kept.repeat_interleave(E // groups, 1), v, -math.inf)
+    want = torch.sort(v, dim=1, descending=True, stable=True).indices[:, :K]
+    idx, _ = route(l, K, score=score, bias=bias if biased else None, num_groups=groups, topk_groups=topk_groups, group_best=best)
+    # (scores of logits a step apart may come to the same 64 bits, or the other way round in their last one: some 1e-16)
+    same = (idx == want).all(1)
+    a, b = v.gather(1, idx), v.gather(1, want)
+    assert ((a - b).abs()[~same] <= 4e-16 * (1 + a.abs()[~same])).all() and (~same).sum() <= (3 if computed else 0)
 
 
 def test_route_of_infinities_and_nan():
