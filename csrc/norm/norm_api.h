@@ -10,7 +10,7 @@ constexpr int kNormMaxHidden = 32768;
 constexpr int kNormScaleBlock = 128;     // channels that share one scale of the fp8 output
 
 // Row r of a [T, H] tensor starts at r * ld elements. All of a call's rows lie alike within 16 bytes: base addresses are
-// equal modulo 16 and so are the row strides in bytes.
+// multiples of 16, and row strides in bytes are equal modulo 16.
 struct NormFwdParams {
   int type, wtype;            // of the rows; of the weight (the rows' type or f32)
   int T, H;

@@ -2,8 +2,10 @@
 //   a = dy w,  n = h r,  dx = dresidual = r (a - n mean(a n)) + dh,  dw = sum over the rows of dy n
 // all in f32, rounded where they are stored. Bound: memory (three or four tensors read, one written). h is read as the
 // forward stored it, which costs dw a relative error of one rounding of h (2^-9 for bf16, about that of storing dw in bf16);
-// for weights in f32 the caller passes x and the residual instead and h is summed again: a tensor more, dw exact to 32 bits. A row is read once and stays in registers; persistent CTAs keep the weights and their part of dw there too, so
-// that dw costs one row of f32 a CTA, summed in a fixed order by a second launch: the same bits from run to run.
+// for weights in f32 the caller passes x and the residual instead and h is summed again: a tensor more, dw exact to 32 bits.
+// Persistent CTAs have the next rows under way in shared memory while they are at one (every thread copies what it will need
+// itself), and keep the weights and their part of dw in registers, so that dw costs one row of f32 a CTA, summed in a fixed
+// order by a second launch: the same bits from run to run.
 #include "norm.cuh"
 
 namespace b200ep {
@@ -11,84 +13,136 @@ namespace norm {
 
 constexpr int kWarpRows = 8;
 
-template <typename T, typename W, int VPT, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : (VPT <= 2 ? 512 : 1024), WARP ? 2 : 1)
-rms_norm_bwd_kernel(const NormBwdParams p) {
-  constexpr int EPV = kEpv<T>;
+template <typename T, typename W, int VPT, bool WARP, bool ALIGNED>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : 1024, 1)
+rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int stages) {
+  constexpr int EPV = kEpv<T>, PAIRS = EPV / 2;
+  extern __shared__ __align__(16) uint4 s_rows[];           // [stage][dy, h, other part of h, dh][vector][thread]
   __shared__ float s_sum[2][32];
   __shared__ float s_dw[WARP ? 32 * VPT * EPV : 1];
   const int H = p.H;
   const int row0 = WARP ? blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
   const int step = WARP ? gridDim.x * kWarpRows : gridDim.x;
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, threads = WARP ? 32 : blockDim.x;
-  const T* dy = static_cast<const T*>(p.dy);
-  const T* dh = static_cast<const T*>(p.dh);
-  const T* h = static_cast<const T*>(p.h);
-  const T* res = static_cast<const T*>(p.res);
-  T* dx = static_cast<T*>(p.dx);
-  const int shift = (int)((reinterpret_cast<uintptr_t>(h + (long long)row0 * p.h_ld) & 15) / sizeof(T));
+  constexpr bool STAGED = kStaged<VPT, WARP>;
+  const bool two = p.res != nullptr, add = p.dh != nullptr;
+  const int shift = ALIGNED ? 0 : (int)((reinterpret_cast<uintptr_t>(static_cast<const T*>(p.h) + (long long)row0 * p.h_ld) & 15) / sizeof(T));
+  const int e_first = tid * EPV - shift, e_next = threads * EPV;         // the thread's first element, and to its next vector's
+  Walk<T> dy(p.dy, p.dy_ld, row0, step, e_first), h(p.h, p.h_ld, row0, step, e_first);
+  Walk<T> res(p.res, p.res_ld, row0, step, e_first), dh(p.dh, p.dh_ld, row0, step, e_first);
+  const uint32_t word = 16u * blockDim.x, plane = VPT * word, at_dh = two ? 3 * plane : 2 * plane, stage_bytes = plane * (2u + two + add);
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_rows) + 16u * threadIdx.x, mine_end = mine + stages * stage_bytes;
+  long long ahead = row0;                                   // the next row to be fetched
+  const auto fetch = [&](uint32_t to) {
+    if constexpr (!STAGED) return;
+    if (ahead < p.T) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (e_first + i * e_next < H) {
+          const int off = i * e_next * (int)sizeof(T), bytes = min(16, (H - e_first - i * e_next) * (int)sizeof(T));
+          fetch_vec<ALIGNED>(to + i * word, dy.at + off, bytes);
+          fetch_vec<ALIGNED>(to + plane + i * word, h.at + off, bytes);
+          if (two) fetch_vec<ALIGNED>(to + 2 * plane + i * word, res.at + off, bytes);
+          if (add) fetch_vec<ALIGNED>(to + at_dh + i * word, dh.at + off, bytes);
+        }
+      dy.at += dy.step;
+      h.at += h.step;
+      res.at += res.step;
+      dh.at += dh.step;
+    }
+    ahead += step;
+    fetch_commit();
+  };
+  for (int k = 0; k < stages; ++k) fetch(mine + k * stage_bytes);
   const bool w_aligned = shift == 0 && (reinterpret_cast<uintptr_t>(p.w) & 15) == 0;
   const float inv_h = 1.f / (float)H;
   WeightVec<T, W> w[VPT];
-  float acc[VPT][EPV];
+  float2 acc[VPT][PAIRS];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    w[i].load(static_cast<const W*>(p.w), (i * threads + tid) * EPV - shift, H, w_aligned);
+    w[i].load(static_cast<const W*>(p.w), e_first + i * e_next, H, w_aligned);
 #pragma unroll
-    for (int j = 0; j < EPV; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < PAIRS; ++j) acc[i][j] = make_float2(0.f, 0.f);
   }
+  // Short rows stay in registers from the sum to the result; of long ones that would cost too many, they are read again.
+  constexpr bool KEEP = WARP || VPT == 1;
+  const int width = WARP ? 32 : block_width();
   int parity = 0;
-  for (long long row = row0; row < p.T; row += step, parity ^= 1) {
-    uint4 gv[VPT], hv[VPT], sv[VPT], rv[VPT];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e0 = (i * threads + tid) * EPV - shift;
-      gv[i] = load_vec(dy + row * p.dy_ld, e0, H);
-      hv[i] = load_vec(h + row * p.h_ld, e0, H);
-      if (res != nullptr) sv[i] = load_vec(res + row * p.res_ld, e0, H);
-      if (dh != nullptr) rv[i] = load_vec(dh + row * p.dh_ld, e0, H);
-    }
-    const float rstd = p.rstd[row];
-    const auto normed = [&](int i, float* n) {
-      unpack<T>(hv[i], n);
-      if (res != nullptr) {
-        float s[EPV];
-        unpack<T>(sv[i], s);
-#pragma unroll
-        for (int j = 0; j < EPV; ++j) n[j] += s[j];
-      }
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) n[j] *= rstd;
+  uint32_t from = mine;
+  const long long out_step = (long long)step * H;
+  long long out = (long long)row0 * H;                      // the row in a contiguous tensor
+  float next_rstd = row0 < p.T ? __ldg(p.rstd + row0) : 0.f;
+  for (long long row = row0; row < p.T; row += step, out += out_step, parity ^= 1) {
+    const float rstd = next_rstd;
+    if (row + step < p.T) next_rstd = __ldg(p.rstd + row + step);
+    if constexpr (STAGED) fetch_wait(stages - 1);
+    const auto vec = [&](uint32_t at, int i, const void* t, long long ld, int e0) {
+      if constexpr (STAGED) return inside<T, ALIGNED>(lds_v4(from + at + i * word), e0);
+      else return load_vec<T, ALIGNED>(static_cast<const T*>(t) + row * ld, e0, H);
     };
-    float c = 0.f;
+    // dy and n = h r of a vector
+    const auto get = [&](int i, int e0, float2 (&g)[PAIRS], float2 (&n)[PAIRS]) {
+      unpack<T>(vec(0, i, p.dy, p.dy_ld, e0), g);
+      unpack<T>(vec(plane, i, p.h, p.h_ld, e0), n);
+      if (two) {
+        float2 s[PAIRS];
+        unpack<T>(vec(2 * plane, i, p.res, p.res_ld, e0), s);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      float g[EPV], n[EPV], wf[EPV];
-      unpack<T>(gv[i], g);
-      normed(i, n);
+        for (int j = 0; j < PAIRS; ++j) n[j] = add2(n[j], s[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j) n[j] = mul2(n[j], both(rstd));
+    };
+    const auto result = [&](int i, int e0, float2 (&g)[PAIRS], const float2 (&n)[PAIRS], const uint4& r4, float c) {
+      float2 wf[PAIRS];
       w[i].get(wf);
 #pragma unroll
-      for (int j = 0; j < EPV; ++j) {
-        const float gn = g[j] * n[j];
-        acc[i][j] += gn;
-        c = fmaf(gn, wf[j], c);
+      for (int j = 0; j < PAIRS; ++j) g[j] = mul2(fma2(n[j], both(-c), mul2(g[j], wf[j])), both(rstd));
+      if (add) {
+        float2 r[PAIRS];
+        unpack<T>(r4, r);
+#pragma unroll
+        for (int j = 0; j < PAIRS; ++j) g[j] = add2(g[j], r[j]);
       }
-    }
-    c = (WARP ? warp_sum(c) : block_sum(c, s_sum[parity])) * inv_h;
+      store_vec<T, ALIGNED>(static_cast<T*>(p.dx) + out, e0, H, pack<T>(g));
+    };
+    float2 g[KEEP ? VPT : 1][PAIRS], n[KEEP ? VPT : 1][PAIRS], c2 = make_float2(0.f, 0.f);
+    uint4 r4[KEEP ? VPT : 1];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float g[EPV], n[EPV], wf[EPV], r[EPV];
-      unpack<T>(gv[i], g);
-      normed(i, n);
+      const int e0 = e_first + i * e_next, k = KEEP ? i : 0;
+      if (e0 >= H) continue;
+      float2 wf[PAIRS];
+      get(i, e0, g[k], n[k]);
+      if (KEEP && add) r4[k] = vec(at_dh, i, p.dh, p.dh_ld, e0);
       w[i].get(wf);
-      if (dh != nullptr) unpack<T>(rv[i], r);
 #pragma unroll
-      for (int j = 0; j < EPV; ++j) {
-        const float d = rstd * (g[j] * wf[j] - n[j] * c);
-        g[j] = dh != nullptr ? d + r[j] : d;
+      for (int j = 0; j < PAIRS; ++j) {
+        const float2 gn = mul2(g[k][j], n[k][j]);
+        acc[i][j] = add2(acc[i][j], gn);
+        c2 = fma2(gn, wf[j], c2);
       }
-      store_vec(dx + row * H, (i * threads + tid) * EPV - shift, H, pack<T>(g));
     }
+    const float c = (WARP ? warp_sum(c2.x + c2.y) : block_sum(c2.x + c2.y, s_sum[parity], width)) * inv_h;
+    if constexpr (KEEP) {
+      fetch(from);         // (this thread's place is free: what it held is in registers)
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int e0 = e_first + i * e_next;
+        if (e0 < H) result(i, e0, g[i], n[i], r4[i], c);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int e0 = e_first + i * e_next;
+        if (e0 >= H) continue;
+        get(i, e0, g[0], n[0]);
+        if (add) r4[0] = vec(at_dh, i, p.dh, p.dh_ld, e0);
+        result(i, e0, g[0], n[0], r4[0], c);
+      }
+      fetch(from);
+    }
+    from = from + stage_bytes == mine_end ? mine : from + stage_bytes;
   }
   if (p.part == nullptr) return;
   float* part = p.part + (long long)blockIdx.x * H;
@@ -102,8 +156,8 @@ rms_norm_bwd_kernel(const NormBwdParams p) {
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
           for (int j = 0; j < EPV; ++j) {
-            const int e = (i * 32 + tid) * EPV - shift + j;
-            if (e >= 0 && e < H) s_dw[e] += acc[i][j];
+            const int e = e_first + i * e_next + j;
+            if (e >= 0 && e < H) s_dw[e] += j % 2 ? acc[i][j / 2].y : acc[i][j / 2].x;
           }
       }
     }
@@ -114,78 +168,80 @@ rms_norm_bwd_kernel(const NormBwdParams p) {
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
       for (int j = 0; j < EPV; ++j) {
-        const int e = (i * threads + tid) * EPV - shift + j;
-        if (e >= 0 && e < H) part[e] = acc[i][j];
+        const int e = e_first + i * e_next + j;
+        if (e >= 0 && e < H) part[e] = j % 2 ? acc[i][j / 2].y : acc[i][j / 2].x;
       }
   }
 }
 
-// dw[e] = sum of the parts in ascending order, 8 strands of them side by side: 32 columns a CTA.
+// dw[e] = sum of the parts: 32 columns a CTA, 32 strands of parts side by side, joined by a tree.
 template <typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 sum_rows_kernel(const float* __restrict__ part, int parts, int H, W* __restrict__ dw) {
-  __shared__ float s[8][32];
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
   float v = 0.f;
   if (e < H) {
-#pragma unroll 4
-    for (int g = strand; g < parts; g += 8) v += part[(long long)g * H + e];
+#pragma unroll 8
+    for (int g = strand; g < parts; g += 32) v += __ldg(part + (long long)g * H + e);
   }
   s[strand][lane] = v;
   __syncthreads();
-  if (strand == 0 && e < H) {
-    v = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v += s[k][lane];
-    dw[e] = from_f<W>(v);
-  }
+  v = warp_sum(s[lane][strand]);
+  if (lane == 0 && blockIdx.x * 32 + strand < H) dw[blockIdx.x * 32 + strand] = from_f<W>(v);
 }
 
-// `grid` null: launches; else only says how many CTAs the launch would have.
-template <typename T, typename W, int VPT, bool WARP>
+// `parts` given: only says how many CTAs the launch will have.
+template <typename T, typename W, int VPT, bool WARP, bool ALIGNED>
 int run_bwd(const NormBwdParams& p, int threads, int* parts, cudaStream_t st) {
-  const auto kern = rms_norm_bwd_kernel<T, W, VPT, WARP>;
-  if (parts != nullptr) {
-    int fit = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, threads, 0) != cudaSuccess || fit < 1) return 2;
-    const int rows = WARP ? kWarpRows : 1;
-    const long long need = ((long long)p.T + rows - 1) / rows;
-    long long grid = (long long)fit * sm_count();
-    const int period = WARP ? 1 : align_period(p.h_ld * (long long)sizeof(T));
-    grid -= grid % period;
-    *parts = (int)(need < grid ? need : grid);
-    return 0;
-  }
-  kern<<<p.parts, threads, 0, st>>>(p);
-  if (p.part != nullptr) sum_rows_kernel<W><<<(p.H + 31) / 32, 256, 0, st>>>(p.part, p.parts, p.H, static_cast<W*>(p.dw));
+  const auto kern = rms_norm_bwd_kernel<T, W, VPT, WARP, ALIGNED>;
+  const int row_bytes = !kStaged<VPT, WARP> ? 0 : VPT * threads * 16 * (2 + (p.res != nullptr) + (p.dh != nullptr));
+  const int rows = WARP ? kWarpRows : 1;
+  const long long need = ((long long)p.T + rows - 1) / rows;
+  static Launch plan;
+  int stages = 0, fit = 0;
+  if (!plan.get(kern, threads, row_bytes, &stages, &fit)) return 2;
+  long long grid = (long long)fit * sm_count();
+  const int period = WARP ? 1 : align_period(p.h_ld * (long long)sizeof(T));
+  grid -= grid % period;
+  if (need <= grid) { grid = need; stages = 1; }
+  if (parts != nullptr) { *parts = (int)grid; return 0; }
+  if (p.part != nullptr && p.parts != (int)grid) return 1;
+  kern<<<(int)grid, threads, stages * row_bytes, st>>>(p, stages);
+  if (p.part != nullptr) sum_rows_kernel<W><<<(p.H + 31) / 32, 1024, 0, st>>>(p.part, p.parts, p.H, static_cast<W*>(p.dw));
   return 0;
 }
 
-template <typename T, typename W>
+template <typename T, typename W, bool ALIGNED>
 int bwd_sized(const NormBwdParams& p, int* parts, cudaStream_t st) {
-  const bool aligned = (reinterpret_cast<uintptr_t>(p.h) & 15) == 0 && (p.h_ld * sizeof(T)) % 16 == 0;
-  const int nvec = (p.H + (aligned ? 0 : kEpv<T> - 1) + kEpv<T> - 1) / kEpv<T>;
-  if (nvec <= 32) return run_bwd<T, W, 1, true>(p, kWarpRows * 32, parts, st);
-  if (nvec <= 64) return run_bwd<T, W, 2, true>(p, kWarpRows * 32, parts, st);
+  const int nvec = (p.H + (ALIGNED ? 0 : kEpv<T> - 1) + kEpv<T> - 1) / kEpv<T>;
+  if (nvec <= 32) return run_bwd<T, W, 1, true, ALIGNED>(p, kWarpRows * 32, parts, st);
+  if (nvec <= 64) return run_bwd<T, W, 2, true, ALIGNED>(p, kWarpRows * 32, parts, st);
   const auto threads = [nvec](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
-  if (nvec <= 1024) return run_bwd<T, W, 2, false>(p, threads(2), parts, st);
-  if (nvec <= 4096) return run_bwd<T, W, 4, false>(p, threads(4), parts, st);
-  return run_bwd<T, W, 9, false>(p, threads(9), parts, st);
+  if (nvec <= 1024) return run_bwd<T, W, 1, false, ALIGNED>(p, threads(1), parts, st);
+  if (nvec <= 2048) return run_bwd<T, W, 2, false, ALIGNED>(p, threads(2), parts, st);
+  if (nvec <= 4096) return run_bwd<T, W, 4, false, ALIGNED>(p, threads(4), parts, st);
+  return run_bwd<T, W, 9, false, ALIGNED>(p, threads(9), parts, st);
+}
+
+template <typename T, typename W>
+int bwd_aligned(const NormBwdParams& p, int* parts, cudaStream_t st) {
+  const bool aligned = p.H % kEpv<T> == 0 && (p.T == 1 || p.h_ld % kEpv<T> == 0);
+  return aligned ? bwd_sized<T, W, true>(p, parts, st) : bwd_sized<T, W, false>(p, parts, st);
 }
 
 static int bwd(const NormBwdParams& p, int* parts, cudaStream_t st) {
   if (p.T < 0 || p.H < 1 || p.H > kNormMaxHidden) return 1;
   if (p.wtype != p.type && p.wtype != ELEM_F32) return 1;
   const long long es = p.type == ELEM_F32 ? 4 : 2;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p.h);
   const auto alike = [&](const void* t, long long ld) {
-    return t == nullptr || ((reinterpret_cast<uintptr_t>(t) ^ at) % 16 == 0 && (ld - p.h_ld) * es % 16 == 0);
+    return t == nullptr || (reinterpret_cast<uintptr_t>(t) % 16 == 0 && (ld - p.h_ld) * es % 16 == 0);
   };
-  if (!alike(p.dy, p.dy_ld) || !alike(p.dh, p.dh_ld) || !alike(p.res, p.res_ld) || !alike(p.dx, p.H) || at % es || reinterpret_cast<uintptr_t>(p.w) % (p.wtype == ELEM_F32 ? 4 : 2)) return 1;
+  if (!alike(p.h, p.h_ld) || !alike(p.dy, p.dy_ld) || !alike(p.dh, p.dh_ld) || !alike(p.res, p.res_ld) || !alike(p.dx, p.H) || reinterpret_cast<uintptr_t>(p.w) % (p.wtype == ELEM_F32 ? 4 : 2)) return 1;
   if (p.T == 0) { if (parts != nullptr) *parts = 0; return 0; }
-  if (p.type == ELEM_BF16) return p.wtype == ELEM_F32 ? bwd_sized<__nv_bfloat16, float>(p, parts, st) : bwd_sized<__nv_bfloat16, __nv_bfloat16>(p, parts, st);
-  if (p.type == ELEM_F16) return p.wtype == ELEM_F32 ? bwd_sized<__half, float>(p, parts, st) : bwd_sized<__half, __half>(p, parts, st);
-  return bwd_sized<float, float>(p, parts, st);
+  if (p.type == ELEM_BF16) return p.wtype == ELEM_F32 ? bwd_aligned<__nv_bfloat16, float>(p, parts, st) : bwd_aligned<__nv_bfloat16, __nv_bfloat16>(p, parts, st);
+  if (p.type == ELEM_F16) return p.wtype == ELEM_F32 ? bwd_aligned<__half, float>(p, parts, st) : bwd_aligned<__half, __half>(p, parts, st);
+  return bwd_aligned<float, float>(p, parts, st);
 }
 
 }  // namespace norm

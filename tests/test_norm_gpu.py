@@ -208,7 +208,7 @@ def test_gradients_are_the_same_bits_again():
 @pytest.mark.parametrize("dt", [BF16, F16, F32])
 @pytest.mark.parametrize("H", [128, 256, 384, 1024, 4096, 7168, 7296, 16512, 32768])
 def test_fp8(H, dt):
-    from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm_fp8
     for T, residual, keep in ((1, True, True), (9, False, False), (333, True, True)):
         x, r, w = _inputs((T, H), dt, F32, residual, seed=T)
         w[:128] = 0                                                # a block of zeros: the least scale
@@ -223,8 +223,7 @@ def test_fp8(H, dt):
         tol = blocks.abs() * (2.0 ** -4 + 120 * _half(F32)) + scale[..., None] * 2.0 ** -10 * 1.001
         assert ((got - blocks).abs() <= tol).all()
         if keep:
-            ref = rms_norm(x, w, residual=r)
-            assert torch.equal(y, ref[0] if residual else ref)
+            _close(y, want, dt)                                    # (rms_norm's may be another of two neighbours: other lanes sum the squares)
         if residual:
             _close(h, hw, dt)
 
