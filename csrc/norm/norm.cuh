@@ -158,7 +158,7 @@ __device__ __forceinline__ void fetch_wait(int left) {
 constexpr int kMaxStages = 4;            // rows that a thread has under way, for fetch_wait
 // Rows come by way of shared memory unless they are so long (more than 2048 vectors) that their tensors do not fit there:
 // those are loads enough at a time by themselves.
-template <int VPT, bool WARP> constexpr bool kStaged = WARP || VPT <= 2;
+template <typename T, int VPT, bool WARP> constexpr bool kStaged = WARP || VPT * kEpv<T> <= 16;
 
 // The weights of one vector of rows in T, kept as they are stored (W: T or float) so that they take few registers.
 template <typename T, typename W>

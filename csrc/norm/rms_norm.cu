@@ -24,7 +24,7 @@ rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
   const int row0 = WARP ? blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
   const int step = WARP ? gridDim.x * kWarpRows : gridDim.x;
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, threads = WARP ? 32 : blockDim.x;
-  constexpr bool STAGED = kStaged<VPT, WARP>;
+  constexpr bool STAGED = kStaged<T, VPT, WARP>;
   const bool add = p.residual != nullptr;
   // (the same for every row of this thread: the grid strides by a multiple of the alignment's period)
   const int shift = ALIGNED ? 0 : (int)((reinterpret_cast<uintptr_t>(static_cast<const T*>(p.x) + (long long)row0 * p.x_ld) & 15) / sizeof(T));
@@ -130,7 +130,7 @@ rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
 template <typename T, typename W, int VPT, bool FP8, bool WARP, bool ALIGNED>
 int launch_fwd(const NormFwdParams& p, int threads, cudaStream_t st) {
   const auto kern = rms_norm_fwd_kernel<T, W, VPT, FP8, WARP, ALIGNED>;
-  const int row_bytes = kStaged<VPT, WARP> ? VPT * threads * 16 * (p.residual != nullptr ? 2 : 1) : 0;
+  const int row_bytes = kStaged<T, VPT, WARP> ? VPT * threads * 16 * (p.residual != nullptr ? 2 : 1) : 0;
   const int rows = WARP ? kWarpRows : 1;
   const long long need = ((long long)p.T + rows - 1) / rows;
   static Launch plan;

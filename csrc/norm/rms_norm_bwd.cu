@@ -24,7 +24,7 @@ rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int stages) {
   const int row0 = WARP ? blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
   const int step = WARP ? gridDim.x * kWarpRows : gridDim.x;
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, threads = WARP ? 32 : blockDim.x;
-  constexpr bool STAGED = kStaged<VPT, WARP>;
+  constexpr bool STAGED = kStaged<T, VPT, WARP>;
   const bool two = p.res != nullptr, add = p.dh != nullptr;
   const int shift = ALIGNED ? 0 : (int)((reinterpret_cast<uintptr_t>(static_cast<const T*>(p.h) + (long long)row0 * p.h_ld) & 15) / sizeof(T));
   const int e_first = tid * EPV - shift, e_next = threads * EPV;         // the thread's first element, and to its next vector's
@@ -195,7 +195,7 @@ sum_rows_kernel(const float* __restrict__ part, int parts, int H, W* __restrict_
 template <typename T, typename W, int VPT, bool WARP, bool ALIGNED>
 int run_bwd(const NormBwdParams& p, int threads, int* parts, cudaStream_t st) {
   const auto kern = rms_norm_bwd_kernel<T, W, VPT, WARP, ALIGNED>;
-  const int row_bytes = !kStaged<VPT, WARP> ? 0 : VPT * threads * 16 * (2 + (p.res != nullptr) + (p.dh != nullptr));
+  const int row_bytes = !kStaged<T, VPT, WARP> ? 0 : VPT * threads * 16 * (2 + (p.res != nullptr) + (p.dh != nullptr));
   const int rows = WARP ? kWarpRows : 1;
   const long long need = ((long long)p.T + rows - 1) / rows;
   static Launch plan;
@@ -218,8 +218,10 @@ int bwd_sized(const NormBwdParams& p, int* parts, cudaStream_t st) {
   if (nvec <= 32) return run_bwd<T, W, 1, true, ALIGNED>(p, kWarpRows * 32, parts, st);
   if (nvec <= 64) return run_bwd<T, W, 2, true, ALIGNED>(p, kWarpRows * 32, parts, st);
   const auto threads = [nvec](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
-  if (nvec <= 1024) return run_bwd<T, W, 1, false, ALIGNED>(p, threads(1), parts, st);
-  if (nvec <= 2048) return run_bwd<T, W, 2, false, ALIGNED>(p, threads(2), parts, st);
+  // up to 512 threads where that goes, so that an SM has two CTAs or more: 16384 x 7168 with 896 threads 224 us, with 448
+  // 198; 16384 x 4096 with 512 102 us, with 256 98.5; 4096 x 8192 in f32 with 1024 83 us, with 512 66
+  if (nvec <= 256) return run_bwd<T, W, 1, false, ALIGNED>(p, threads(1), parts, st);
+  if (nvec <= (sizeof(T) == 4 ? 1024 : 2048)) return run_bwd<T, W, 2, false, ALIGNED>(p, threads(2), parts, st);
   if (nvec <= 4096) return run_bwd<T, W, 4, false, ALIGNED>(p, threads(4), parts, st);
   return run_bwd<T, W, 9, false, ALIGNED>(p, threads(9), parts, st);
 }

@@ -29,7 +29,11 @@ __global__ void __launch_bounds__(256)
 balance_count_kernel(const BalanceParams p, int rows_per) {
   __shared__ int s_count[kRouterMaxExperts];
   __shared__ int s_rows;
-  const int E = p.E, K = p.K;
+  stream_order_next();
+  const int E = p.E, K = p.K, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // a warp looks at as many rows at a time as have their choices in its lanes
+  const int rows_at_once = 32 / K, sub = lane / K, choice = lane - sub * K;
+  const uint32_t one_row = K == 32 ? 0xffffffffu : (1u << K) - 1;
   const long long lo = (long long)blockIdx.x * rows_per, hi = min(lo + rows_per, (long long)p.T);
   for (long long at = lo; at < hi;) {
     if (p.seq_off != nullptr) {                             // (rows outside all sequences at either end are passed over at once)
@@ -46,13 +50,17 @@ balance_count_kernel(const BalanceParams p, int rows_per) {
       for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
       if (threadIdx.x == 0) s_rows = 0;
       __syncthreads();
-      for (long long t = at + (threadIdx.x >> 5); t < end; t += blockDim.x >> 5) {
-        const int lane = threadIdx.x & 31;
-        const long long i = lane < K ? p.idx[t * K + lane] : -1;
+      int live = 0;
+      for (long long t0 = at + warp * rows_at_once; t0 < end; t0 += (long long)(blockDim.x >> 5) * rows_at_once) {
+        const long long t = t0 + sub;
+        const long long i = sub < rows_at_once && t < end ? __ldg(p.idx + t * K + choice) : -1;
         const bool ok = i >= 0 && i < E;
         if (ok) atomicAdd(s_count + (int)i, 1);
-        if (__any_sync(0xffffffffu, ok) && lane == 0) atomicAdd(&s_rows, 1);
+        const uint32_t some = __ballot_sync(0xffffffffu, ok);
+        if (choice == 0 && sub < rows_at_once && (some >> (sub * K) & one_row)) ++live;
       }
+      live = __reduce_add_sync(0xffffffffu, live);
+      if (lane == 0 && live) atomicAdd(&s_rows, live);
       __syncthreads();
       for (int e = threadIdx.x; e < E; e += blockDim.x)
         if (s_count[e]) atomicAdd(p.counts + (long long)b * E + e, s_count[e]);
@@ -76,23 +84,35 @@ __device__ __forceinline__ float sequence_share(const BalanceParams& p) {
   return 1.f / (float)max(1, s_live);
 }
 
-// What a warp holds of the row it looks at.
+// A row as it is read: this lane's logits, and whether it has a choice (lane k looks at choice k).
+template <typename L, int VPL>
+struct Raw {
+  float l[VPL];
+  bool chose = false;
+  __device__ __forceinline__ void load(const BalanceParams& a, long long t, int lane) {
+    const long long i = lane < a.K ? a.idx[t * a.K + lane] : -1;
+    chose = i >= 0 && i < a.E;
+    const L* row = static_cast<const L*>(a.logits) + t * a.ld;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) l[k] = k * 32 + lane < a.E ? logit(row + k * 32 + lane) : -INFINITY;
+  }
+};
+
+// What a warp makes of it.
 template <typename L, int VPL>
 struct Row {
   float p[VPL];              // share of the scores
   float s[VPL];              // sigmoid: 1 - score
   float lse, F;
   // false: the row takes no part
-  __device__ __forceinline__ bool load(const BalanceParams& a, long long t, const float* f, int lane) {
-    const long long i = lane < a.K ? a.idx[t * a.K + lane] : -1;
-    const L* row = static_cast<const L*>(a.logits) + t * a.ld;
+  __device__ __forceinline__ bool of(const BalanceParams& a, const Raw<L, VPL>& raw, const float* f) {
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
-      p[k] = k * 32 + lane < a.E ? logit(row + k * 32 + lane) : -INFINITY;
+      p[k] = raw.l[k];
       top = nan_max(p[k], top);
     }
-    if (!__any_sync(0xffffffffu, i >= 0 && i < a.E)) return false;
+    if (!__any_sync(0xffffffffu, raw.chose)) return false;
     float sum = 0.f;
     lse = 0.f;
     if (a.score == SCORE_SOFTMAX) {
@@ -145,18 +165,23 @@ struct Walk {
 constexpr int kBalanceWarps = 8;
 
 template <typename L, int VPL>
-__global__ void __launch_bounds__(kBalanceWarps * 32)
+__global__ void __launch_bounds__(kBalanceWarps * 32, VPL <= 8 ? 4 : 2)
 balance_loss_kernel(const BalanceParams p, int rows_per_warp) {
   __shared__ double s_part[kBalanceWarps];
   __shared__ bool s_last;
+  stream_order_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float per_sequence = sequence_share(p);
   const long long lo = ((long long)blockIdx.x * kBalanceWarps + warp) * rows_per_warp, hi = min(lo + rows_per_warp, (long long)p.T);
   Walk<VPL> at;
+  Raw<L, VPL> raw, next;
   Row<L, VPL> row;
   double mine = 0.0;
+  if (lo < hi) next.load(p, lo, lane);
   for (long long t = lo; t < hi; ++t) {
-    if (!at.to(p, t, per_sequence, lane) || !row.load(p, t, at.f, lane)) continue;
+    raw = next;
+    if (t + 1 < hi) next.load(p, t + 1, lane);              // (under way while this row is looked at)
+    if (!at.to(p, t, per_sequence, lane) || !row.of(p, raw, at.f)) continue;
     mine += (double)at.share * ((double)p.coeff * (double)row.F + (double)p.z_coeff * (double)row.lse * (double)row.lse);
   }
   if (lane == 0) s_part[warp] = mine;
@@ -169,17 +194,23 @@ balance_loss_kernel(const BalanceParams p, int rows_per_warp) {
     s_last = atomicAdd(p.counts + (long long)p.B * p.E + p.B, 1) == (int)gridDim.x - 1;
   }
   __syncthreads();
-  if (!s_last || warp != 0) return;
+  if (!s_last) return;
   __threadfence();
   double v = 0.0;
-  for (int k = lane; k < (int)gridDim.x; k += 32) v += __ldcg(p.part + k);
+  for (int k = threadIdx.x; k < (int)gridDim.x; k += kBalanceWarps * 32) v += __ldcg(p.part + k);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane == 0) *p.loss = (float)v;
+  __syncthreads();                                          // (thread 0 has read s_part by now)
+  if (lane == 0) s_part[warp] = v;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  v = 0.0;
+  for (int k = 0; k < kBalanceWarps; ++k) v += s_part[k];
+  *p.loss = (float)v;
 }
 
 template <typename L, int VPL>
-__global__ void __launch_bounds__(kBalanceWarps * 32)
+__global__ void __launch_bounds__(kBalanceWarps * 32, VPL <= 8 ? 4 : 2)
 balance_bwd_kernel(const BalanceBwdParams a, int rows_per_warp) {
   const BalanceParams& p = a.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -187,10 +218,14 @@ balance_bwd_kernel(const BalanceBwdParams a, int rows_per_warp) {
   const float g = *a.dloss;
   const long long lo = ((long long)blockIdx.x * kBalanceWarps + warp) * rows_per_warp, hi = min(lo + rows_per_warp, (long long)p.T);
   Walk<VPL> at;
+  Raw<L, VPL> raw, next;
   Row<L, VPL> row;
+  if (lo < hi) next.load(p, lo, lane);
   for (long long t = lo; t < hi; ++t) {
+    raw = next;
+    if (t + 1 < hi) next.load(p, t + 1, lane);
     L* out = static_cast<L*>(a.dlogits) + t * p.E;
-    const bool in = at.to(p, t, per_sequence, lane) && row.load(p, t, at.f, lane);
+    const bool in = at.to(p, t, per_sequence, lane) && row.of(p, raw, at.f);
     const float c = g * at.share * p.coeff, z = 2.f * g * at.share * p.z_coeff * (in ? row.lse : 0.f);
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
@@ -218,8 +253,7 @@ inline int ctas(int T) {
 
 template <typename L, int VPL>
 int forward_sized(const BalanceParams& p, cudaStream_t st) {
-  balance_loss_kernel<L, VPL><<<balance_ctas(p), kBalanceWarps * 32, 0, st>>>(p, rows_a_warp(p.T));
-  return 0;
+  return launch_ordered(balance_loss_kernel<L, VPL>, dim3(balance_ctas(p)), dim3(kBalanceWarps * 32), 0, st, 1, p, rows_a_warp(p.T)) == cudaSuccess ? 0 : 2;
 }
 template <typename L, int VPL>
 int backward_sized(const BalanceBwdParams& a, cudaStream_t st) {
