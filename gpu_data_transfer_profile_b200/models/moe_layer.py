@@ -3,7 +3,9 @@
 The reference's "model" is exactly this loop with a random router stand-in
 (`DeepEP_Megatron/test_deepep_moe_dispatch_combine.py:731-742,766-815`); here it is an
 `nn.Module` with a learnable router so that forward AND backward run (dispatch and combine
-are each other's backward, expert GEMMs have dgrad/wgrad).
+are each other's backward, expert GEMMs have dgrad/wgrad). Optional, off by default: the norm in front of it with the
+residual's addition (`ops.norm`), the choice of experts by other scores, with a bias and in groups, and the loss that
+keeps it balanced (`ops.router`).
 """
 from __future__ import annotations
 
@@ -13,6 +15,8 @@ import torch
 from torch.autograd.forward_ad import unpack_dual
 
 from .. import _ext
+from ..ops import norm as N
+from ..ops import router as R
 from .experts import build_experts
 from .experts_tcgen05 import Tcgen05GroupedExperts
 from .token_dispatcher import B200TokenDispatcher
@@ -80,13 +84,38 @@ def _carries_more(t: Optional[torch.Tensor]) -> bool:
 
 
 class MoELayer(torch.nn.Module):
+    """`score`, `num_groups`, `topk_groups`, `group_best`, `renormalize` and `route_scale` are `ops.router.route`'s;
+    `expert_bias=True` adds the buffer `expert_bias` (f32 [E], zeros) that the choice is made with: the program moves it
+    towards a balanced load. With `balance_coeff` or `z_coeff`, a forward pass with gradients leaves
+    `ops.router.balance_loss` of its (this rank's) choices in `aux_loss`, for the program to add to its loss; without
+    gradients `aux_loss` is None. A choice of -1 (a router logit of -inf) goes to no expert.
+    `norm=True` puts `ops.norm.rms_norm` with the parameter `norm_weight` in front: `forward` then takes the residual as
+    well and returns (output, hidden_states + residual)."""
+
     def __init__(self, hidden_size: int, ffn_hidden_size: int, num_experts: int, topk: int, group=None, *,
                  ep_size: int = 1, ep_rank: int = 0, dtype=torch.bfloat16, activation: str = "swiglu",
                  expert_backend: str = "auto", dispatcher_mode: str = "fused", world=None, device="cuda",
-                 fuse_combine: bool = True, use_fp8: bool = False):
+                 fuse_combine: bool = True, use_fp8: bool = False, score: str = "softmax", num_groups: int = 1,
+                 topk_groups: Optional[int] = None, group_best: int = 1, renormalize: bool = True, route_scale: float = 1.0,
+                 expert_bias: bool = False, balance_coeff: float = 0.0, z_coeff: float = 0.0, norm: bool = False,
+                 norm_eps: float = 1e-6):
         super().__init__()
         if num_experts % ep_size:
             raise ValueError("num_experts must be divisible by the EP size")
+        if score not in R.SCORES:
+            raise ValueError(f"unsupported score {score!r}; expected one of {R.SCORES}")
+        if z_coeff and score != "softmax":
+            raise ValueError("z_coeff goes with softmax scores")
+        self._choice = dict(score=score, num_groups=num_groups, topk_groups=topk_groups, group_best=group_best,
+                            renormalize=renormalize, scale=route_scale)
+        self._balance = dict(score=score, coeff=balance_coeff, z_coeff=z_coeff) if balance_coeff or z_coeff else None
+        # the plain softmax router keeps the launches (and the higher derivatives) of its own
+        self._plain_choice = (score == "softmax" and num_groups == 1 and renormalize and route_scale == 1.0
+                              and not expert_bias and self._balance is None)
+        self.register_buffer("expert_bias", torch.zeros(num_experts, dtype=torch.float32, device=device) if expert_bias else None)
+        self.register_parameter("norm_weight", torch.nn.Parameter(torch.ones(hidden_size, dtype=dtype, device=device)) if norm else None)
+        self.norm_eps = norm_eps
+        self.aux_loss: Optional[torch.Tensor] = None
         self.hidden_size, self.num_experts, self.topk = hidden_size, num_experts, topk
         self.fuse_combine = fuse_combine
         self.num_local_experts = num_experts // ep_size
@@ -99,6 +128,35 @@ class MoELayer(torch.nn.Module):
         self.use_fp8 = bool(use_fp8) and getattr(self.experts, "use_fp8", False)
         self.dispatcher = B200TokenDispatcher(group, self.num_local_experts, num_experts,
                                               ep_rank * self.num_local_experts, mode=dispatcher_mode, world=world)
+
+    def __getstate__(self):
+        # (a loss that hangs on a graph can neither be copied nor stored)
+        return {**self.__dict__, "aux_loss": None}
+
+    def _fused_logits(self, x) -> bool:
+        """Whether the router's own kernel may stand in for its product with these rows."""
+        return (type(x) is torch.Tensor and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous()
+                and x.data_ptr() % 16 == 0 and x.shape[1] % 8 == 0 and x.device == self.router.weight.device
+                and _plain_linear(self.router) and self.router.weight.shape == (self.num_experts, x.shape[1]))
+
+    def _choose(self, hidden_states: torch.Tensor, router_logits: Optional[torch.Tensor], inference: bool,
+                seq_off: Optional[torch.Tensor]):
+        """(expert ids, weights) by `ops.router`, and the balance loss of a pass with gradients."""
+        l = router_logits
+        if l is None:
+            if inference and hidden_states.is_cuda and self._fused_logits(hidden_states):
+                l = _ext.load().router_logits(hidden_states, self.router.weight)
+            else:
+                l = self.router(hidden_states.float())
+        if l.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            l = l.float()
+        if topk_softmax_router is not _OWN_ROUTER:
+            idx, w = topk_softmax_router(l, self.topk)
+        else:
+            idx, w = R.route(l, self.topk, bias=self.expert_bias, **self._choice)
+        if self._balance is not None and torch.is_grad_enabled():
+            self.aux_loss = R.balance_loss(l, idx, seq_off=seq_off, **self._balance)
+        return idx, w
 
     def _route(self, hidden_states: torch.Tensor, router_logits: Optional[torch.Tensor], inference: bool):
         """(expert ids, weights). For inference the router runs on this library's kernels (f32 like the
@@ -116,26 +174,51 @@ class MoELayer(torch.nn.Module):
             return topk_softmax_router(l, K)
         if router_logits is None:
             x = hidden_states
-            if (type(x) is torch.Tensor and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous()
-                    and x.data_ptr() % 16 == 0 and x.shape[1] % 8 == 0 and x.device == self.router.weight.device
-                    and _plain_linear(self.router) and self.router.weight.shape == (E, x.shape[1])):
+            if self._fused_logits(x):
                 return C.route(x, self.router.weight, K)
             router_logits = self.router(x.float())
         if type(router_logits) is not torch.Tensor or router_logits.dim() != 2 or router_logits.shape[1] > C.ROUTER_MAX_EXPERTS:
             return topk_softmax_router(router_logits, K)
         return C.topk_softmax(router_logits.float().contiguous(), K)
 
-    def forward(self, hidden_states: torch.Tensor, router_logits: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """hidden_states [T,H]; router_logits [T,E] override the learnable router when given."""
+    def forward(self, hidden_states: torch.Tensor, router_logits: Optional[torch.Tensor] = None,
+                residual: Optional[torch.Tensor] = None, seq_off: Optional[torch.Tensor] = None):
+        """hidden_states [T,H]; router_logits [T,E] override the learnable router when given. residual [T,H] (with
+        `norm=True` only) is added before the norm: -> (output, sum) in that case, output otherwise. seq_off: the
+        sequences that the rows are packed from, for the balance loss."""
+        self.aux_loss = None
+        if self.norm_weight is None:
+            if residual is not None:
+                raise ValueError("a residual goes with norm=True")
+            return self._mix(hidden_states, router_logits, seq_off, None)
+        rows = None
+        if (self.use_fp8 and self.dispatcher.mode == "fused" and hidden_states.dtype == torch.bfloat16
+                and not torch.is_grad_enabled() and _unchanged(self.dispatcher, _OWN_DISPATCHER)
+                and _unchanged(self.experts, _OWN_EXPERTS)):
+            # the exchange's cast is part of the norm; the router sees the rows before it
+            rows, x, h = N.rms_norm_fp8(hidden_states, self.norm_weight, residual=residual, eps=self.norm_eps, keep=True)
+        elif residual is None:
+            x, h = N.rms_norm(hidden_states, self.norm_weight, eps=self.norm_eps), None
+        else:
+            x, h = N.rms_norm(hidden_states, self.norm_weight, residual=residual, eps=self.norm_eps)
+        return self._mix(x, router_logits, seq_off, rows), hidden_states if h is None else h
+
+    def _mix(self, hidden_states: torch.Tensor, router_logits: Optional[torch.Tensor], seq_off: Optional[torch.Tensor], fp8_rows):
+        """Router, dispatch, experts, combine. fp8_rows: the same rows as (e4m3, scales), where they were made before."""
         inference = not (torch.is_grad_enabled() or topk_softmax_router is not _OWN_ROUTER or _carries_more(hidden_states)
                          or _carries_more(router_logits) or _carries_more(getattr(self.router, "weight", None)))
-        idx, probs = self._route(hidden_states, router_logits, inference)
+        if self._plain_choice:
+            idx, probs = self._route(hidden_states, router_logits, inference)
+        else:
+            idx, probs = self._choose(hidden_states, router_logits, inference, seq_off)
         if (inference and self.dispatcher.mode == "fused" and hidden_states.dtype == torch.bfloat16
                 and (self.use_fp8 or self.fuse_combine)
                 and _unchanged(self.dispatcher, _OWN_DISPATCHER) and _unchanged(self.experts, _OWN_EXPERTS)):
             # Inference: the rows are consumed where they arrive, before the next dispatch can be issued on this
             # stream, so they need no copy of their own, and the GEMMs take their tile lists from the device.
-            rows, row_probs, handle = self.dispatcher.dispatch_in_place(hidden_states, idx, probs, use_fp8=self.use_fp8)
+            rows, row_probs, handle = self.dispatcher.dispatch_in_place(
+                hidden_states if fp8_rows is None else fp8_rows, idx, probs, use_fp8=self.use_fp8 and fp8_rows is None,
+                masked=not self._plain_choice)
             if self.use_fp8:
                 El = self.num_local_experts
                 off = handle.meta[2 + El: 2 + El + El + 1]

@@ -122,20 +122,22 @@ class B200TokenDispatcher:
         return rows, tpe, row_probs
 
     @torch.no_grad()
-    def dispatch_in_place(self, hidden_states, token_indices, token_probs, use_fp8: bool = False):
+    def dispatch_in_place(self, hidden_states, token_indices, token_probs, use_fp8: bool = False, masked: bool = False):
         """Forward-only, fused mode, for a caller that consumes the rows at once on the current stream: they (and
         nothing else) stay views of the receive region, valid until the second next dispatch. Returns (rows, or
         (e4m3 rows, scales) with use_fp8, one probability per row, handle).
         A group of one receives exactly its own items, so the host need not wait for the receive count;
-        every index must then name an expert (no -1)."""
+        every index must then name an expert: with masked=True there may be -1 among them, and it waits.
+        hidden_states may be (e4m3 rows, scales), as `Buffer.dispatch` takes them, with use_fp8=False."""
         if self.mode != "fused":
             raise ValueError("dispatch_in_place is offered by the fused (expert-grouped) dispatcher")
-        x = hidden_states.contiguous()
-        buf = A.get_buffer(self.group, A.get_hidden_bytes(x), self.world)
+        x = tuple(t.contiguous() for t in hidden_states) if isinstance(hidden_states, tuple) else hidden_states.contiguous()
+        first = x[0] if isinstance(x, tuple) else x
+        buf = A.get_buffer(self.group, A.get_hidden_bytes(first), self.world)
         idx = token_indices.contiguous()
         worst = 0
-        if buf.group_size == 1:
-            H, K = x.shape[1], idx.shape[1]
+        if buf.group_size == 1 and not masked:
+            H, K = first.shape[1], idx.shape[1]
             items = idx.numel()
             # (a region too small for them takes the counted path, which names the overflow)
             worst = items if 0 < items <= buf._get_carve(self.num_experts, K, H, H * 2, H * 2).cap else 0
