@@ -7,6 +7,7 @@
 // v is compared in 64 bits where it is computed (a bias, or a sum of two in groups): neighbours among some hundred scores lie
 // so close that 32 bits choose another expert for one token in some ten thousand. Where v ranks as the logits do, their own
 // 32 bits are compared. Not a number ranks above everything, as in torch.topk.
+#include <atomic>
 #include "route.cuh"
 
 namespace b200ep {
@@ -172,8 +173,9 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, const L* row, c
 // are left to choose_exactly. 256 sigmoid scores with a bias: about one token in 200 is settled, one in 1000 for its groups.
 //   kLogit16: 16-bit logits rank by themselves; the low half of a key is the expert, the lowest highest: always told apart
 //   kLogit32: 32-bit logits rank by themselves, but for the low bits that the place in the lane takes
-//   kComputed: scores and a bias in 32 bits, also but for those low bits
-enum Mode : int { kLogit16 = 0, kLogit32 = 1, kComputed = 2 };
+//   kSigmoid, kSoftmax: computed values, scores and a bias in 32 bits, also but for those low bits
+enum Mode : int { kLogit16 = 0, kLogit32 = 1, kSigmoid = 2, kSoftmax = 3 };
+constexpr bool computed(int mode) { return mode >= kSigmoid; }
 
 // A float's bits in the order of its values (-0 just below 0). Keys up to kAbsent, that of -inf, stand for nothing.
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -220,13 +222,13 @@ __device__ __forceinline__ float quick_sigmoid(float x) {
 // The values that are compared, as they are defined: of 64 bits where they are computed.
 template <int MODE>
 struct Defined {
-  using V = typename std::conditional<MODE == kComputed, double, float>::type;
-  using KEY = typename std::conditional<MODE == kComputed, Key64, Key32>::type;
+  using V = typename std::conditional<computed(MODE), double, float>::type;
+  using KEY = typename std::conditional<computed(MODE), Key64, Key32>::type;
   V top = 0, total = 0;
   // by the whole warp
   template <typename L>
   __device__ __forceinline__ void row(const RouteParams& p, const L* row) {
-    if (MODE != kComputed || p.score != SCORE_SOFTMAX) return;
+    if (MODE != kSoftmax) return;
     const int lane = threadIdx.x & 31;
     top = -INFINITY;
     for (int j = lane; j < p.E; j += 32) {
@@ -245,9 +247,9 @@ struct Defined {
   template <typename L>
   __device__ __forceinline__ V of(const RouteParams& p, const L* row, int e) const {
     V v = (V)logit(row + e);
-    if constexpr (MODE == kComputed) {
+    if constexpr (computed(MODE)) {
       if (v == (V)-INFINITY) return v;
-      v = p.score == SCORE_SOFTMAX ? exp(v - top) / total : 1.0 / (1.0 + exp(-v));
+      v = MODE == kSoftmax ? exp(v - top) / total : 1.0 / (1.0 + exp(-v));
       if (p.bias != nullptr) v += (V)__ldg(p.bias + e);
     }
     return v;
@@ -343,184 +345,233 @@ template <> struct Four<__half> {
   }
 };
 
+// A lane's experts where a warp has a token.
+template <int VPL>
+struct Share {
+  int group, e0, n;          // its group, first expert, and how many it has
+  float bias[VPL], most_bias;
+  __device__ __forceinline__ Share(const RouteParams& p, const Groups& gr, bool computed) {
+    const int lane = threadIdx.x & 31, sub = lane & (gr.lanes - 1);
+    group = lane / gr.lanes;
+    e0 = group * gr.size + sub * gr.chunk;
+    n = group < gr.count ? max(0, min(gr.chunk, gr.size - sub * gr.chunk)) : 0;
+    most_bias = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      bias[i] = computed && p.bias != nullptr && i < n ? __ldg(p.bias + e0 + i) : 0.f;
+      if (fabsf(bias[i]) < INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
+    }
+    if (computed) most_bias = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_bias)));
+  }
+};
+
+// One token by one warp: the expert of lane k's choice, -1 for none (lanes from K on hold anything). With softmax also the
+// largest logit and the sum of the exponentials of the distances to it.
+template <typename L, int VPL, int MODE>
+__device__ __forceinline__ int choose(const RouteParams& p, const Groups& gr, const Share<VPL>& mine, const L* row, float& top, float& sum) {
+  const int lane = threadIdx.x & 31, group = mine.group;
+  const bool soft = MODE == kSoftmax || (!computed(MODE) && p.score == SCORE_SOFTMAX);
+  constexpr int LOW = MODE == kLogit16 ? 0 : kLog2<VPL>;    // bits of a key that say where it came from
+  constexpr uint32_t MASK = (1u << LOW) - 1;
+  float l[VPL];
+  bool loaded = false;
+  if constexpr (VPL % 4 == 0) {
+    if (gr.vec) {
+#pragma unroll
+      for (int i = 0; i < VPL; i += 4) {
+        l[i] = l[i + 1] = l[i + 2] = l[i + 3] = -INFINITY;
+        if (i < mine.n) Four<L>::get(row + mine.e0 + i, l + i);
+      }
+      loaded = true;
+    }
+  }
+  if (!loaded) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) l[i] = i < mine.n ? logit(row + mine.e0 + i) : -INFINITY;
+  }
+  if (soft) {
+    top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) top = nan_max(l[i], top);
+    top = warp_max(top);
+    if (top == -INFINITY) top = 0.f;                      // no expert is available: all scores are 0
+  }
+  uint32_t key[VPL];
+  float margin = 0.f;                                     // how far a key's value may be from the one it stands for
+  bool odd = false;                                       // not a number among logits that are compared as they are
+  if constexpr (computed(MODE)) {
+    float s[VPL], unit = 1.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) s[i] = MODE == kSoftmax ? __expf(l[i] - top) : quick_sigmoid(l[i]);
+    if constexpr (MODE == kSoftmax) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) sum += s[i];
+      sum = warp_sum(sum);
+      unit = reciprocal(sum);
+    }
+    // A sigmoid is off by 2^-21 of at most 1. A softmax score p has its exponential off by 2 units in the last place and, for
+    // the distance d to the maximum, by 2 d 2^-24 of itself, which p = e^-d / sum makes less than 2^-24 of the largest, 1 / sum;
+    // and a sum of VPL + 5 roundings and those of its terms: 2^-18 of the largest covers all. The sum with the bias is
+    // rounded once, its key has LOW bits of its own.
+    margin = (MODE == kSoftmax ? 0x1p-18f * unit : 0x1p-21f) + (float)(1 + (1 << LOW)) * 0x1p-23f * (unit + mine.most_bias);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const float c = l[i] == -INFINITY ? -INFINITY : fmaf(s[i], unit, mine.bias[i]);
+      key[i] = (order_of(c) & ~MASK) | (uint32_t)(VPL - 1 - i);        // (a sum that is not a number has the highest)
+    }
+  } else {
+    if (soft) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) sum += __expf(l[i] - top);
+      sum = warp_sum(sum);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      odd = odd || l[i] != l[i];
+      if constexpr (MODE == kLogit16) {
+        key[i] = order16(l[i] + 0.f, row);
+        key[i] |= key[i] > kAbsent ? (uint32_t)(0xffff - (mine.e0 + i)) : 0u;
+      } else {
+        key[i] = (order_of(l[i]) & ~MASK) | (uint32_t)(VPL - 1 - i);
+      }
+    }
+  }
+  // whether two values, the first with the higher key, are in this order for certain
+  const auto apart = [&](uint32_t high, uint32_t low) {
+    if (MODE == kLogit16 || low <= kAbsent) return true;
+    if (MODE == kLogit32) return (high & ~MASK) > (low & ~MASK) && !(low >= (0x7fffffffu & ~MASK) && high <= (0x80000000u | MASK));      // (-0 is 0)
+    return Key32::value(high) - Key32::value(low) > 2.f * margin;
+  };
+  sort_keys(key);
+  bool exact = gr.exact || (!computed(MODE) && __any_sync(0xffffffffu, odd));
+  if (gr.count > 1) {
+    // the group's two highest, in all of its lanes
+    uint32_t a = key[0], b = key[1];
+    for (int o = gr.lanes >> 1; o > 0; o >>= 1) {
+      const uint32_t c = __shfl_xor_sync(0xffffffffu, a, o), d = __shfl_xor_sync(0xffffffffu, b, o);
+      b = max(min(a, c), max(b, d));
+      a = max(a, c);
+    }
+    // its value as a key that is its own: the low bits say which group (a logit of 16 bits has them already), lowest first
+    if (computed(MODE) && p.group_best == 2 && b > kAbsent) a = order_of(Key32::value(a) + Key32::value(b));
+    if (MODE != kLogit16 && a > kAbsent) a = (a & ~gr.mask) | (gr.mask - (uint32_t)group);
+    uint32_t left = a, last = 0u;
+    for (int k = 0; k < p.topk_groups; ++k) {
+      last = __reduce_max_sync(0xffffffffu, left);
+      if (left == last) left = 0u;
+    }
+    bool kept = left == 0u;
+    if constexpr (MODE != kLogit16) {
+      // (two values of either side, their sums' rounding and the keys' own bits; -0 and 0 lie within a step of 2^-149)
+      const uint32_t next = __reduce_max_sync(0xffffffffu, left);
+      const uint32_t low = gr.mask | MASK;
+      const float about = computed(MODE) ? 4.f * margin + (float)(2 + 2 * low) * 0x1p-23f * fabsf(Key32::value(last)) : 0.f;
+      const bool close = next > kAbsent && (MODE == kLogit32 ? (last & ~low) == (next & ~low) || (next >= (0x7fffffffu & ~low) && last <= (0x80000000u | low))
+                                                            : !(Key32::value(last) - Key32::value(next) > about));
+      if (close && !exact) {
+        // those near the last one that stays are looked at again, the others are in or out
+        bool in, near;
+        if (MODE == kLogit32) {
+          const uint32_t zero = 0x80000000u & ~low, at = (last & ~low) == (0x7fffffffu & ~low) ? zero : last & ~low;
+          const uint32_t me = (a & ~low) == (0x7fffffffu & ~low) ? zero : a & ~low;
+          near = a > kAbsent && me == at;
+          in = a > kAbsent && me > at;
+        } else {
+          const float off = Key32::value(a) - Key32::value(last);
+          near = a > kAbsent && !(fabsf(off) > about);
+          in = a > kAbsent && off > about;
+        }
+        const uint32_t first = __ballot_sync(0xffffffffu, (lane & (gr.lanes - 1)) == 0 && group < gr.count);
+        const uint32_t in_lanes = __ballot_sync(0xffffffffu, in) & first, near_lanes = __ballot_sync(0xffffffffu, near) & first;
+        uint32_t among = 0u;
+        for (uint32_t m = near_lanes; m != 0u; m &= m - 1) among |= 1u << ((__ffs(m) - 1) / gr.lanes);
+        const uint32_t stay = settle_groups<L, MODE>(p, row, gr.size, among, p.topk_groups - __popc(in_lanes));
+        kept = in || (near && (stay >> group & 1));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = kept ? key[i] : 0u;
+  }
+  // The lane whose first key is the highest leaves it, and the expert, in the choice's place. Two lanes with the same key
+  // leave theirs in one: the count says so.
+  __shared__ uint2 s_pick[8][32];
+  uint2* const picks = s_pick[threadIdx.x >> 5];
+  uint32_t high = 0u;
+  int n = 0, given = 0;
+  const auto give = [&] {
+    if (key[0] == high) {
+      picks[n] = make_uint2(key[0], MODE == kLogit16 ? 0xffffu - (key[0] & 0xffffu) : (uint32_t)(mine.e0 + VPL - 1) - (key[0] & MASK));
+      ++given;
+#pragma unroll
+      for (int i = 0; i + 1 < VPL; ++i) key[i] = key[i + 1];
+      key[VPL - 1] = 0u;
+    }
+  };
+  __syncwarp();
+#pragma unroll 1
+  for (; n < p.K; ++n) {
+    high = __reduce_max_sync(0xffffffffu, key[0]);
+    if (high <= kAbsent) break;
+    give();
+  }
+  __syncwarp();
+  uint2 pick = picks[lane];
+  int e = lane < n ? (int)pick.y : -1;
+  if constexpr (MODE != kLogit16) {
+    uint32_t next = n == p.K ? __reduce_max_sync(0xffffffffu, key[0]) : 0u;
+    const uint32_t follows = __shfl_down_sync(0xffffffffu, pick.x, 1), after = lane + 1 < n ? follows : next;
+    const bool doubt = lane < n && !apart(pick.x, after);
+    const int total = __reduce_add_sync(0xffffffffu, given);
+    if (total != n) exact = true;
+    if (__any_sync(0xffffffffu, doubt) && !exact) {
+      // behind the last choice, the values that may change places with it
+      while (n < 32 && !apart(high, next)) {
+        high = next;
+        give();
+        ++n;
+        next = __reduce_max_sync(0xffffffffu, key[0]);
+      }
+      __syncwarp();
+      pick = picks[lane];
+      if (!apart(high, next) || (int)__reduce_add_sync(0xffffffffu, given) != n) exact = true;       // (32 of them and more)
+      else e = settle<L, MODE>(p, row, (int)pick.y, n);
+    }
+  }
+  if (exact) e = choose_exactly<L, VPL, typename Defined<MODE>::KEY>(p, row, gr);
+  return e;
+}
+
+// Weights of a token's choices, lane k's of choice k: e < 0 for none.
+template <typename L>
+__device__ __forceinline__ void store_choice(const RouteParams& p, const L* row, long long t, int k, int e, float top, float sum) {
+  const bool soft = p.score == SCORE_SOFTMAX;
+  float l = 0.f, s = 0.f;
+  if (e >= 0) {
+    l = logit(row + e);
+    s = soft ? expf(l - top) * reciprocal(sum) : reciprocal(1.f + expf(-l));
+  }
+  float chosen = s;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
+  if (k < p.K) {
+    p.idx[t * p.K + k] = e;
+    p.w[t * p.K + k] = e < 0 ? 0.f : (p.renorm ? s * reciprocal(chosen + kSumEps) : s) * p.scale;
+    if (p.aux != nullptr && !soft) p.aux[t * p.K + k] = l;
+  }
+  if (p.aux != nullptr && soft && !p.renorm && k < 2) p.aux[t * 2 + k] = k == 0 ? top : (sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+}
+
 template <typename L, int VPL, int MODE>
 __global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2)
 route_kernel(const __grid_constant__ RouteParams p, const __grid_constant__ Groups gr) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const bool soft = p.score == SCORE_SOFTMAX;
-  constexpr int LOW = MODE == kLogit16 ? 0 : kLog2<VPL>;    // bits of a key that say where it came from
-  constexpr uint32_t MASK = (1u << LOW) - 1;
-  const int group = lane / gr.lanes, sub = lane & (gr.lanes - 1);
-  const int e0 = group * gr.size + sub * gr.chunk;          // the lane's first expert, and how many it has
-  const int mine_n = group < gr.count ? max(0, min(gr.chunk, gr.size - sub * gr.chunk)) : 0;
-  float bias[VPL], most_bias = 0.f;
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    bias[i] = MODE == kComputed && p.bias != nullptr && i < mine_n ? __ldg(p.bias + e0 + i) : 0.f;
-    if (fabsf(bias[i]) < INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
-  }
-  if (MODE == kComputed) most_bias = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_bias)));
+  const Share<VPL> mine(p, gr, computed(MODE));
   for (long long t = (long long)blockIdx.x * warps + warp; t < p.T; t += (long long)gridDim.x * warps) {
     const L* row = static_cast<const L*>(p.logits) + t * p.ld;
-    float l[VPL];
     float top = 0.f, sum = 0.f;
-    bool loaded = false;
-    if constexpr (VPL % 4 == 0) {
-      if (gr.vec) {
-#pragma unroll
-        for (int i = 0; i < VPL; i += 4) {
-          l[i] = l[i + 1] = l[i + 2] = l[i + 3] = -INFINITY;
-          if (i < mine_n) Four<L>::get(row + e0 + i, l + i);
-        }
-        loaded = true;
-      }
-    }
-    if (!loaded) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) l[i] = i < mine_n ? logit(row + e0 + i) : -INFINITY;
-    }
-    if (soft) {
-      top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) top = nan_max(l[i], top);
-      top = warp_max(top);
-      if (top == -INFINITY) top = 0.f;                      // no expert is available: all scores are 0
-    }
-    uint32_t key[VPL];
-    float margin = 0.f;                                     // how far a key's value may be from the one it stands for
-    bool odd = false;                                       // not a number among logits that are compared as they are
-    if constexpr (MODE == kComputed) {
-      float s[VPL], unit = 1.f;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) s[i] = soft ? __expf(l[i] - top) : quick_sigmoid(l[i]);
-      if (soft) {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) sum += s[i];
-        sum = warp_sum(sum);
-        unit = reciprocal(sum);
-      }
-      // A sigmoid is off by 2^-21 of at most 1. A softmax score p has its exponential off by 2 units in the last place and, for
-      // the distance d to the maximum, by 2 d 2^-24 of itself, which p = e^-d / sum makes less than 2^-24 of the largest, 1 / sum;
-      // and a sum of VPL + 5 roundings and those of its terms: 2^-18 of the largest covers all. The sum with the bias is
-      // rounded once, its key has LOW bits of its own.
-      margin = (soft ? 0x1p-18f * unit : 0x1p-21f) + (float)(1 + (1 << LOW)) * 0x1p-23f * (unit + most_bias);
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const float c = l[i] == -INFINITY ? -INFINITY : fmaf(s[i], unit, bias[i]);
-        key[i] = (order_of(c) & ~MASK) | (uint32_t)(VPL - 1 - i);        // (a sum that is not a number has the highest)
-      }
-    } else {
-      if (soft) {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) sum += __expf(l[i] - top);
-        sum = warp_sum(sum);
-      }
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        odd = odd || l[i] != l[i];
-        if constexpr (MODE == kLogit16) {
-          key[i] = order16(l[i] + 0.f, row);
-          key[i] |= key[i] > kAbsent ? (uint32_t)(0xffff - (e0 + i)) : 0u;
-        } else {
-          key[i] = (order_of(l[i]) & ~MASK) | (uint32_t)(VPL - 1 - i);
-        }
-      }
-    }
-    // whether two values, the first with the higher key, are in this order for certain
-    const auto apart = [&](uint32_t high, uint32_t low) {
-      if (MODE == kLogit16 || low <= kAbsent) return true;
-      if (MODE == kLogit32) return (high & ~MASK) > (low & ~MASK) && !(low >= (0x7fffffffu & ~MASK) && high <= (0x80000000u | MASK));      // (-0 is 0)
-      return Key32::value(high) - Key32::value(low) > 2.f * margin;
-    };
-    sort_keys(key);
-    bool exact = gr.exact || (MODE != kComputed && __any_sync(0xffffffffu, odd));
-    if (gr.count > 1) {
-      // the group's two highest, in all of its lanes
-      uint32_t a = key[0], b = key[1];
-      for (int o = gr.lanes >> 1; o > 0; o >>= 1) {
-        const uint32_t c = __shfl_xor_sync(0xffffffffu, a, o), d = __shfl_xor_sync(0xffffffffu, b, o);
-        b = max(min(a, c), max(b, d));
-        a = max(a, c);
-      }
-      // its value as a key that is its own: the low bits say which group (a logit of 16 bits has them already), lowest first
-      if (MODE == kComputed && p.group_best == 2 && b > kAbsent) a = order_of(Key32::value(a) + Key32::value(b));
-      if (MODE != kLogit16 && a > kAbsent) a = (a & ~gr.mask) | (gr.mask - (uint32_t)group);
-      uint32_t left = a, last = 0u;
-      for (int k = 0; k < p.topk_groups; ++k) {
-        last = __reduce_max_sync(0xffffffffu, left);
-        if (left == last) left = 0u;
-      }
-      bool kept = left == 0u;
-      if constexpr (MODE != kLogit16) {
-        // (two values of either side, their sums' rounding and the keys' own bits; -0 and 0 lie within a step of 2^-149)
-        const uint32_t next = __reduce_max_sync(0xffffffffu, left);
-        const uint32_t low = gr.mask | MASK;
-        const float about = MODE == kComputed ? 4.f * margin + (float)(2 + 2 * low) * 0x1p-23f * fabsf(Key32::value(last)) : 0.f;
-        const bool close = next > kAbsent && (MODE == kLogit32 ? (last & ~low) == (next & ~low) || (next >= (0x7fffffffu & ~low) && last <= (0x80000000u | low))
-                                                              : !(Key32::value(last) - Key32::value(next) > about));
-        if (close && !exact) {
-          // those near the last one that stays are looked at again, the others are in or out
-          bool in, near;
-          if (MODE == kLogit32) {
-            const uint32_t zero = 0x80000000u & ~low, at = (last & ~low) == (0x7fffffffu & ~low) ? zero : last & ~low;
-            const uint32_t me = (a & ~low) == (0x7fffffffu & ~low) ? zero : a & ~low;
-            near = a > kAbsent && me == at;
-            in = a > kAbsent && me > at;
-          } else {
-            const float off = Key32::value(a) - Key32::value(last);
-            near = a > kAbsent && !(fabsf(off) > about);
-            in = a > kAbsent && off > about;
-          }
-          const uint32_t first = __ballot_sync(0xffffffffu, (lane & (gr.lanes - 1)) == 0 && group < gr.count);
-          const uint32_t in_lanes = __ballot_sync(0xffffffffu, in) & first, near_lanes = __ballot_sync(0xffffffffu, near) & first;
-          uint32_t among = 0u;
-          for (uint32_t m = near_lanes; m != 0u; m &= m - 1) among |= 1u << ((__ffs(m) - 1) / gr.lanes);
-          const uint32_t stay = settle_groups<L, MODE>(p, row, gr.size, among, p.topk_groups - __popc(in_lanes));
-          kept = in || (near && (stay >> group & 1));
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) key[i] = kept ? key[i] : 0u;
-    }
-    // lane k keeps choice k; behind the last one, the values that may change places with it
-    uint32_t mine = 0u, high = 0u;
-    int from = 0, n = 0;
-    for (; n < 32; ++n) {
-      const uint32_t before = high;
-      high = __reduce_max_sync(0xffffffffu, key[0]);
-      if (high <= kAbsent || (n >= p.K && apart(before, high))) break;
-      const int at = __ffs(__ballot_sync(0xffffffffu, key[0] == high)) - 1;
-      if (lane == n) { mine = high; from = at; }
-      if (lane == at) {
-#pragma unroll
-        for (int i = 0; i + 1 < VPL; ++i) key[i] = key[i + 1];
-        key[VPL - 1] = 0u;
-      }
-    }
-    int mine_e = __shfl_sync(0xffffffffu, e0, from) + VPL - 1 - (int)(mine & MASK);
-    if (MODE == kLogit16) mine_e = 0xffff - (int)(mine & 0xffffu);
-    if (lane >= n) mine_e = -1;
-    if constexpr (MODE != kLogit16) {
-      const uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
-      const bool doubt = n > p.K || __any_sync(0xffffffffu, lane + 1 < n && !apart(mine, after));
-      // (32 of them, and the next may be as close)
-      exact = exact || (n == 32 && !apart(__shfl_sync(0xffffffffu, mine, 31), __reduce_max_sync(0xffffffffu, key[0])));
-      if (doubt && !exact) mine_e = settle<L, MODE>(p, row, mine_e, n);
-    }
-    if (exact) mine_e = choose_exactly<L, VPL, typename Defined<MODE>::KEY>(p, row, gr);
-    if (lane >= p.K) mine_e = -1;
-    float mine_l = 0.f, s = 0.f;
-    if (mine_e >= 0) {
-      mine_l = logit(row + mine_e);
-      s = soft ? expf(mine_l - top) * reciprocal(sum) : reciprocal(1.f + expf(-mine_l));
-    }
-    const float chosen = warp_sum(s);
-    if (lane < p.K) {
-      p.idx[t * p.K + lane] = mine_e;
-      p.w[t * p.K + lane] = mine_e < 0 ? 0.f : (p.renorm ? s * reciprocal(chosen + kSumEps) : s) * p.scale;
-      if (p.aux != nullptr && !soft) p.aux[t * p.K + lane] = mine_l;
-    }
-    if (p.aux != nullptr && soft && !p.renorm && lane < 2) p.aux[t * 2 + lane] = lane == 0 ? top : (sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+    int e = choose<L, VPL, MODE>(p, gr, mine, row, top, sum);
+    if (lane >= p.K) e = -1;
+    store_choice<L>(p, row, t, lane, e, top, sum);
   }
 }
 
@@ -578,34 +629,41 @@ template <typename L, int VPL, int MODE>
 int launch_sized(const RouteParams& p, const Groups& g, cudaStream_t st) {
   const int warps = p.T < 1184 ? 1 : 8;
   const auto kern = route_kernel<L, VPL, MODE>;
-  int fit = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, warps * 32, 0) != cudaSuccess || fit < 1) return 2;
+  static std::atomic<int> fits[2];                          // CTAs per SM with 1 and with 8 warps; 0: not asked yet
+  int fit = fits[warps > 1].load(std::memory_order_relaxed);
+  if (fit == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, warps * 32, 0) != cudaSuccess || fit < 1) return 2;
+    fits[warps > 1].store(fit, std::memory_order_relaxed);
+  }
   const long long need = ((long long)p.T + warps - 1) / warps, most = (long long)fit * sm_count();
   kern<<<(int)(need < most ? need : most), warps * 32, 0, st>>>(p, g);
   return 0;
 }
-template <typename L, int MODE>
-int launch_mode(const RouteParams& p, cudaStream_t st) {
+// The groups of a choice over a warp's lanes.
+template <typename L>
+Groups lay_groups(const RouteParams& p, bool told_apart) {
   Groups g{};
-  g.count = p.topk_groups < p.groups ? p.groups : 1;
+  g.told = p.topk_groups < p.groups ? p.groups : 1;
+  g.count = told_apart ? g.told : 1;
   g.size = p.E / g.count;
-  g.told = g.count;
-  g.magic = ((1 << 20) + g.size - 1) / g.size;
-  const auto lay = [&g] {
-    g.lanes = 32;
-    while (g.lanes * g.count > 32) g.lanes >>= 1;
-    g.chunk = (g.size + g.lanes - 1) / g.lanes;
-  };
-  lay();
-  if (g.chunk > 32) {
-    g.exact = true;
-    g.count = 1;
-    g.size = p.E;
-    lay();
-  }
+  const int told_size = p.E / g.told;
+  g.magic = ((1 << 20) + told_size - 1) / told_size;
+  g.lanes = 32;
+  while (g.lanes * g.count > 32) g.lanes >>= 1;
+  g.chunk = (g.size + g.lanes - 1) / g.lanes;
   g.mask = 0u;
   while ((int)g.mask + 1 < g.count) g.mask = 2 * g.mask + 1;
   g.vec = g.chunk % 4 == 0 && g.size % g.chunk == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(L)) == 0;
+  return g;
+}
+
+template <typename L, int MODE>
+int launch_mode(const RouteParams& p, cudaStream_t st) {
+  Groups g = lay_groups<L>(p, true);
+  if (g.chunk > 32) {
+    g = lay_groups<L>(p, false);
+    g.exact = true;
+  }
   if (g.chunk <= 2) return launch_sized<L, 2, MODE>(p, g, st);
   if (g.chunk <= 4) return launch_sized<L, 4, MODE>(p, g, st);
   if (g.chunk <= 8) return launch_sized<L, 8, MODE>(p, g, st);
@@ -614,8 +672,8 @@ int launch_mode(const RouteParams& p, cudaStream_t st) {
 }
 template <typename L>
 int launch_typed(const RouteParams& p, cudaStream_t st) {
-  const bool computed = p.bias != nullptr || (p.topk_groups < p.groups && p.group_best == 2);
-  if (computed) return launch_mode<L, kComputed>(p, st);
+  if (p.bias != nullptr || (p.topk_groups < p.groups && p.group_best == 2))
+    return p.score == SCORE_SOFTMAX ? launch_mode<L, kSoftmax>(p, st) : launch_mode<L, kSigmoid>(p, st);
   return launch_mode<L, sizeof(L) == 2 ? kLogit16 : kLogit32>(p, st);
 }
 
