@@ -17,6 +17,7 @@ constexpr int kWarpRows = 8;             // rows of a CTA at a time where a warp
 template <typename T, typename W, int VPT, bool FP8, bool WARP, bool ALIGNED>
 __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : 1024, WARP ? 2 : 1)
 rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
+  stream_order_wait();
   constexpr int EPV = kEpv<T>, PAIRS = EPV / 2;
   extern __shared__ __align__(16) uint4 s_rows[];           // [stage][x, residual][vector][thread]
   __shared__ float s_sum[2][32];
@@ -140,8 +141,7 @@ int launch_fwd(const NormFwdParams& p, int threads, cudaStream_t st) {
   const int period = WARP ? 1 : align_period(p.x_ld * (long long)sizeof(T));      // (8 rows at a time are a multiple of every period)
   grid -= grid % period;
   if (need <= grid) { grid = need; stages = 1; }
-  kern<<<(int)grid, threads, stages * row_bytes, st>>>(p, stages);
-  return 0;
+  return launch_ordered(kern, dim3((unsigned)grid), dim3(threads), stages * row_bytes, st, 1, p, stages) == cudaSuccess ? 0 : 2;
 }
 
 template <typename T, typename W, bool FP8, bool ALIGNED>

@@ -16,6 +16,8 @@ constexpr int kWarpRows = 8;
 template <typename T, typename W, int VPT, bool WARP, bool ALIGNED>
 __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : 1024, 1)
 rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int stages) {
+  stream_order_wait();
+  stream_order_next();
   constexpr int EPV = kEpv<T>, PAIRS = EPV / 2;
   extern __shared__ __align__(16) uint4 s_rows[];           // [stage][dy, h, other part of h, dh][vector][thread]
   __shared__ float s_sum[2][32];
@@ -178,6 +180,8 @@ rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int stages) {
 template <typename W>
 __global__ void __launch_bounds__(1024)
 sum_rows_kernel(const float* __restrict__ part, int parts, int H, W* __restrict__ dw) {
+  stream_order_wait();
+  stream_order_next();
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, strand = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
   float v = 0.f;
@@ -207,9 +211,9 @@ int run_bwd(const NormBwdParams& p, int threads, int* parts, cudaStream_t st) {
   if (need <= grid) { grid = need; stages = 1; }
   if (parts != nullptr) { *parts = (int)grid; return 0; }
   if (p.part != nullptr && p.parts != (int)grid) return 1;
-  kern<<<(int)grid, threads, stages * row_bytes, st>>>(p, stages);
-  if (p.part != nullptr) sum_rows_kernel<W><<<(p.H + 31) / 32, 1024, 0, st>>>(p.part, p.parts, p.H, static_cast<W*>(p.dw));
-  return 0;
+  if (launch_ordered(kern, dim3((unsigned)grid), dim3(threads), stages * row_bytes, st, 1, p, stages) != cudaSuccess) return 2;
+  if (p.part == nullptr) return 0;
+  return launch_ordered(sum_rows_kernel<W>, dim3((p.H + 31) / 32), dim3(1024), 0, st, 1, p.part, p.parts, p.H, static_cast<W*>(p.dw)) == cudaSuccess ? 0 : 2;
 }
 
 template <typename T, typename W, bool ALIGNED>

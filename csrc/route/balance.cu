@@ -170,6 +170,7 @@ balance_loss_kernel(const BalanceParams p, int rows_per_warp) {
   __shared__ double s_part[kBalanceWarps];
   __shared__ bool s_last;
   stream_order_wait();
+  stream_order_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float per_sequence = sequence_share(p);
   const long long lo = ((long long)blockIdx.x * kBalanceWarps + warp) * rows_per_warp, hi = min(lo + rows_per_warp, (long long)p.T);
@@ -212,6 +213,8 @@ balance_loss_kernel(const BalanceParams p, int rows_per_warp) {
 template <typename L, int VPL>
 __global__ void __launch_bounds__(kBalanceWarps * 32, VPL <= 8 ? 4 : 2)
 balance_bwd_kernel(const BalanceBwdParams a, int rows_per_warp) {
+  stream_order_wait();
+  stream_order_next();
   const BalanceParams& p = a.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float per_sequence = sequence_share(p);
@@ -257,8 +260,7 @@ int forward_sized(const BalanceParams& p, cudaStream_t st) {
 }
 template <typename L, int VPL>
 int backward_sized(const BalanceBwdParams& a, cudaStream_t st) {
-  balance_bwd_kernel<L, VPL><<<balance_ctas(a.f), kBalanceWarps * 32, 0, st>>>(a, rows_a_warp(a.f.T));
-  return 0;
+  return launch_ordered(balance_bwd_kernel<L, VPL>, dim3(balance_ctas(a.f)), dim3(kBalanceWarps * 32), 0, st, 1, a, rows_a_warp(a.f.T)) == cudaSuccess ? 0 : 2;
 }
 
 #define B200EP_BY_SIZE(E, CALL)              \

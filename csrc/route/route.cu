@@ -564,6 +564,7 @@ __device__ __forceinline__ void store_choice(const RouteParams& p, const L* row,
 template <typename L, int VPL, int MODE>
 __global__ void __launch_bounds__(256, VPL <= 8 ? 4 : 2)
 route_kernel(const __grid_constant__ RouteParams p, const __grid_constant__ Groups gr) {
+  stream_order_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const Share<VPL> mine(p, gr, computed(MODE));
   for (long long t = (long long)blockIdx.x * warps + warp; t < p.T; t += (long long)gridDim.x * warps) {
@@ -583,6 +584,8 @@ route_kernel(const __grid_constant__ RouteParams p, const __grid_constant__ Grou
 template <typename L>
 __global__ void __launch_bounds__(256)
 route_bwd_kernel(const RouteBwdParams p) {
+  stream_order_wait();
+  stream_order_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, E = p.E;
   const long long t = (long long)blockIdx.x * (blockDim.x >> 5) + warp;
   if (t >= p.T) return;
@@ -636,8 +639,7 @@ int launch_sized(const RouteParams& p, const Groups& g, cudaStream_t st) {
     fits[warps > 1].store(fit, std::memory_order_relaxed);
   }
   const long long need = ((long long)p.T + warps - 1) / warps, most = (long long)fit * sm_count();
-  kern<<<(int)(need < most ? need : most), warps * 32, 0, st>>>(p, g);
-  return 0;
+  return launch_ordered(kern, dim3((unsigned)(need < most ? need : most)), dim3(warps * 32), 0, st, 1, p, g) == cudaSuccess ? 0 : 2;
 }
 // The groups of a choice over a warp's lanes.
 template <typename L>
@@ -693,10 +695,8 @@ int launch_route_bwd(const RouteBwdParams& p, cudaStream_t st) {
   if (p.T < 0 || p.E < 1 || p.K < 1 || p.K > kRouteMaxTopk || !(p.scale > 0.f)) return 1;
   if (p.T == 0) return 0;
   const int grid = (int)(((long long)p.T + 7) / 8);
-  if (p.type == ELEM_BF16) route::route_bwd_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
-  else if (p.type == ELEM_F16) route::route_bwd_kernel<__half><<<grid, 256, 0, st>>>(p);
-  else route::route_bwd_kernel<float><<<grid, 256, 0, st>>>(p);
-  return 0;
+  const auto kern = p.type == ELEM_BF16 ? route::route_bwd_kernel<__nv_bfloat16> : p.type == ELEM_F16 ? route::route_bwd_kernel<__half> : route::route_bwd_kernel<float>;
+  return launch_ordered(kern, dim3(grid), dim3(256), 0, st, 1, p) == cudaSuccess ? 0 : 2;
 }
 
 }  // namespace b200ep
