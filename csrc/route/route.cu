@@ -613,7 +613,8 @@ route_bwd_kernel(const RouteBwdParams p) {
   } else {
     const float u = e >= 0 ? p.w[t * p.K + lane] / p.scale : 0.f;
     const float dot = warp_sum(u * g);
-    d = u * (g - dot);
+    // (renormalised, their sum is 1 but for roundings, which g times the sum takes out: no gradient where there is one choice)
+    d = u * ((p.renorm ? g * warp_sum(u) : g) - dot);
     if (!p.renorm) {
       const L* row = static_cast<const L*>(p.logits) + t * p.ld;
       const float top = p.aux[t * 2], inv = p.aux[t * 2 + 1];

@@ -3,7 +3,11 @@
 h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight  over the last dimension, in f32; h and y are rounded once, where
 they are stored (y is that of the sum before its rounding). Rows are bf16, f16 or f32, of 1 to 32768 elements, any number of
 leading dimensions; weights are of the rows' type or f32 (others are taken to f32 first). Two-dimensional inputs may have
-rows further apart than their length; other strides are copied.
+rows further apart than their length; other strides are copied. A row's result does not depend on the rows beside it; where
+rows are no multiple of 16 bytes long, it may be a rounding apart with the place within 16 bytes at which the row begins.
+
+Calls can be captured into CUDA graphs, with their gradients too; as with every torch operation, let go of eager graphs of
+the same leaves before a backward pass is captured.
 """
 from __future__ import annotations
 

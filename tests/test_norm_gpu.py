@@ -307,3 +307,27 @@ def test_stream_and_graph():
         assert torch.equal(y, yr) and torch.equal(h, hr) and all(torch.equal(p, q_) for p, q_ in zip(grads, want))
         (q2, s2), _, _ = rms_norm_fp8(x2, w2)
         assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(sc, s2)
+
+
+@pytest.mark.parametrize("H", [32768, 1407])
+def test_offsets_beyond_32_bits(H):
+    """More elements than 32 bits count: the last rows are what they are by themselves (in rows that begin at another place
+    within 16 bytes other lanes sum, and a result may be the neighbouring one)."""
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
+    T = (1 << 31) // H + 100
+    x = torch.empty(T, H, dtype=BF16, device="cuda").normal_().requires_grad_(True)
+    w = torch.ones(H, device="cuda", requires_grad=True)
+    tail = x[-64:].detach().clone().requires_grad_(True)
+    y = rms_norm(x, w)
+    want = rms_norm(tail, w)
+    _close(y[-64:].detach(), _wide(tail.detach(), w.detach(), None, 1e-6)[0], BF16)
+    dx, dw = torch.autograd.grad(y, (x, w), x.detach().flip(0))
+    dt = torch.autograd.grad(want, tail, x[:64].detach().flip(0))[0]
+    # a value of its own size, one step of bf16 apart at most; where it cancels, 32-bit roundings of terms below 64
+    assert ((dx[-64:].double() - dt.double()).abs() <= dt.double().abs() * 2.0 ** -7 + 64 * 100 * 2.0 ** -24).all() and dw.isfinite().all()
+    del dx, y
+    if H % 128 == 0:
+        with torch.no_grad():
+            (q, s), _, h = rms_norm_fp8(x, w, residual=x)
+            (q2, s2), _, h2 = rms_norm_fp8(tail, w, residual=tail)
+        assert torch.equal(q[-64:].view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s[-64:], s2) and torch.equal(h[-64:], h2)

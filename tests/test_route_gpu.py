@@ -255,6 +255,14 @@ def test_route_strides_and_empty():
     assert torch.autograd.grad(w.sum(), e)[0].shape == (0, 64)
 
 
+def test_route_gradient_of_one_renormalised_choice_is_zero():
+    from gpu_data_transfer_profile_b200.ops.router import route
+    l = torch.randn(500, 64, device="cuda", requires_grad=True)
+    w = route(l, 1, scale=2.5)[1]
+    assert (w == 2.5).float().mean() > 0.5 and (w - 2.5).abs().max() <= 2.5 * 4 * U
+    assert (torch.autograd.grad(w, l, torch.randn(500, 1, device="cuda"))[0] == 0).all()
+
+
 def test_route_gradient_against_differences():
     from gpu_data_transfer_profile_b200.ops.router import route
     g = torch.Generator(device="cuda").manual_seed(0)
@@ -458,3 +466,27 @@ def test_stream_and_graph():
         for _, a, out in graphs:
             want = step(a.detach().clone().requires_grad_(True))
             assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_offsets_beyond_32_bits():
+    """More logits than 32 bits count: the last rows are what they are by themselves."""
+    from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
+    T, E = (1 << 31) // 1024 + 300, 1024
+    l = torch.empty(T, E, dtype=BF16, device="cuda").normal_()
+    tail = l[-400:].clone()
+    kw = dict(score="sigmoid", num_groups=8, topk_groups=4, group_best=2)
+    idx, w = route(l, 8, **kw)
+    want = route(tail, 8, **kw)
+    assert torch.equal(idx[-400:], want[0]) and torch.equal(w[-400:], want[1])
+    off = torch.tensor([T - 400, T], dtype=torch.int32, device="cuda")
+    # (the same sums of 64 bits, in other CTAs)
+    assert balance_loss(l, idx, score="sigmoid", seq_off=off).item() == pytest.approx(balance_loss(tail, want[0], score="sigmoid").item(), rel=1e-6)
+    del idx, w
+    l.requires_grad_(True)
+    idx, w = route(l, 8, **kw)
+    g = torch.autograd.grad(w, l, torch.ones_like(w))[0]
+    t = tail.requires_grad_(True)
+    assert torch.equal(g[-400:], torch.autograd.grad(route(t, 8, **kw)[1], t, torch.ones(400, 8, device="cuda"))[0])
+    del g, w
+    g = torch.autograd.grad(balance_loss(l, idx, score="sigmoid", seq_off=off), l)[0]
+    assert (g[:1000] == 0).all() and g[-400:].float().norm() > 0 and g[-401].abs().max() == 0
