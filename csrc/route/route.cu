@@ -7,6 +7,10 @@
 // v is compared in 64 bits where it is computed (a bias, or a sum of two in groups): neighbours among some hundred scores lie
 // so close that 32 bits choose another expert for one token in some ten thousand. Where v ranks as the logits do, their own
 // 32 bits are compared. Not a number ranks above everything, as in torch.topk.
+// A warp has a token: its lanes hold runs of neighbouring experts of one group, so that a group's best are found inside a
+// lane and a few shuffles. Bound: instructions, about 780 a token of 256 experts in 8 groups (16383 of them, top-8, sigmoid
+// with a bias: 18.3 us on one B200, 70 % of the issue slots; every value in 64 bits: 55.5), for few tokens latency (128: 4.4,
+// or 6.7 with a token that needs 64 bits). The logits are read once.
 #include <atomic>
 #include "route.cuh"
 
@@ -170,7 +174,7 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, const L* row, c
 // maximum of the lanes' first keys. How far a key's value may be from the one it stands for is known; where neighbours
 // among the choices, and the values after the last one, lie closer than that, they are compared again as they are defined
 // (settle: one lane each), so are groups that close to the last one that stays (settle_groups). More than 32 such values
-// are left to choose_exactly. 256 sigmoid scores with a bias: about one token in 200 is settled, one in 1000 for its groups.
+// are left to choose_exactly. 256 sigmoid scores with a bias: about one token in 500 is settled, one in 4000 for its groups.
 //   kLogit16: 16-bit logits rank by themselves; the low half of a key is the expert, the lowest highest: always told apart
 //   kLogit32: 32-bit logits rank by themselves, but for the low bits that the place in the lane takes
 //   kSigmoid, kSoftmax: computed values, scores and a bias in 32 bits, also but for those low bits
@@ -581,6 +585,8 @@ route_kernel(const __grid_constant__ RouteParams p, const __grid_constant__ Grou
 //                           h_k = (g_k - sum_j g_j s_j / S) / S with S = sum_j s_j + 1e-20
 //   softmax, renormalised:  the weights are a softmax over the chosen logits: d l_k = u_k (g_k - sum_j u_j g_j), u = w / scale
 //   softmax as it is:       d l_e = p_e ([e chosen] g_e - sum_j g_j p_j) for every expert
+// Bound: memory, the zeros written to [T, E] above all; only the last form reads the logits again. 16384 x 256 in f32: 6.3 us
+// (2.7 TB/s).
 template <typename L>
 __global__ void __launch_bounds__(256)
 route_bwd_kernel(const RouteBwdParams p) {
