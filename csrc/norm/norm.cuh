@@ -101,15 +101,15 @@ __device__ __forceinline__ uint4 inside(uint4 v, int e0) {
   return v;
 }
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store_vec(T* row, int e0, int H, const uint4& v) {
+__device__ __forceinline__ void store_vec(char* at, int e0, int H, const uint4& v) {
   if (ALIGNED ? e0 < H : whole<T>(e0, H)) {
-    st_global_v4(row + e0, v);
+    st_global_v4(at, v);
   } else if constexpr (!ALIGNED) {
     union { uint4 v; T e[kEpv<T>]; } u;
     u.v = v;
 #pragma unroll
     for (int j = 0; j < kEpv<T>; ++j)
-      if (e0 + j >= 0 && e0 + j < H) row[e0 + j] = u.e[j];
+      if (e0 + j >= 0 && e0 + j < H) reinterpret_cast<T*>(at)[j] = u.e[j];
   }
 }
 
@@ -137,13 +137,13 @@ __device__ __forceinline__ uint4 lds_v4(uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
 }
-// One tensor's rows as a thread walks over them: the address of its first vector in the next row to be fetched.
+// One tensor's rows as a thread walks over them: the address of its first vector in the next row that it looks at.
 template <typename T>
 struct Walk {
-  const char* at;
+  char* at;
   long long step;
   __device__ __forceinline__ Walk(const void* t, long long ld, long long row0, int step_rows, int e0) {
-    at = reinterpret_cast<const char*>(static_cast<const T*>(t) + row0 * ld + e0);
+    at = const_cast<char*>(reinterpret_cast<const char*>(static_cast<const T*>(t) + row0 * ld + e0));
     step = (long long)step_rows * ld * (long long)sizeof(T);
   }
 };

@@ -61,9 +61,16 @@ rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
   const int width = WARP ? 32 : block_width();
   int parity = 0;
   uint32_t from = mine;
+  // Where the results go: addresses that are moved along (60000 x 257 34 us, 51 with them made anew from the row's offset), but
+  // in the fp8 form, whose registers that costs (8191 x 7168 94.4 us, 91.6 from the offset).
+  Walk<T> y(p.y, H, row0, step, e_first), sum(p.h, H, row0, step, e_first);
   const long long out_step = (long long)step * H;
-  long long out = (long long)row0 * H;                      // the row in a contiguous tensor
-  for (long long row = row0; row < p.T; row += step, out += out_step, parity ^= 1) {
+  long long out = (long long)row0 * H;
+  const auto at = [&](const Walk<T>& w, void* t, int i) {
+    if constexpr (FP8) return reinterpret_cast<char*>(static_cast<T*>(t) + out + e_first + i * e_next);
+    else return w.at + i * e_next * (int)sizeof(T);
+  };
+  for (long long row = row0; row < p.T; row += step, out += out_step, y.at += y.step, sum.at += sum.step, parity ^= 1) {
     if constexpr (STAGED) fetch_wait(stages - 1);
     float2 h[VPT][PAIRS], ss = make_float2(0.f, 0.f);
 #pragma unroll
@@ -92,7 +99,7 @@ rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
     from = from + stage_bytes == mine_end ? mine : from + stage_bytes;
     if (add) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) store_vec<T, ALIGNED>(static_cast<T*>(p.h) + out, e_first + i * e_next, H, pack<T>(h[i]));
+      for (int i = 0; i < VPT; ++i) store_vec<T, ALIGNED>(at(sum, p.h, i), e_first + i * e_next, H, pack<T>(h[i]));
     }
     const float rstd = inverse_root(fmaf(total, inv_h, p.eps));
     if (tid == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
@@ -103,7 +110,7 @@ rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
       w[i].get(wf);
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j) h[i][j] = mul2(mul2(h[i][j], both(rstd)), wf[j]);
-      if (!FP8 || p.y != nullptr) store_vec<T, ALIGNED>(static_cast<T*>(p.y) + out, e0, H, pack<T>(h[i]));
+      if (!FP8 || p.y != nullptr) store_vec<T, ALIGNED>(at(y, p.y, i), e0, H, pack<T>(h[i]));
       if constexpr (FP8) {
         // (the 128 / EPV lanes of a block are neighbours and all in or all out of the row)
         float amax = 0.f;

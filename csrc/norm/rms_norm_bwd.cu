@@ -107,7 +107,7 @@ rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int stages) {
 #pragma unroll
         for (int j = 0; j < PAIRS; ++j) g[j] = add2(g[j], r[j]);
       }
-      store_vec<T, ALIGNED>(static_cast<T*>(p.dx) + out, e0, H, pack<T>(g));
+      store_vec<T, ALIGNED>(reinterpret_cast<char*>(static_cast<T*>(p.dx) + out + e0), e0, H, pack<T>(g));
     };
     float2 g[KEEP ? VPT : 1][PAIRS], n[KEEP ? VPT : 1][PAIRS], c2 = make_float2(0.f, 0.f);
     uint4 r4[KEEP ? VPT : 1];

@@ -1,0 +1,46 @@
+"""Norm, routing and balance loss without a GPU: what is refused before anything is launched, and their cases."""
+import random
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
+
+
+def test_tensors_on_the_cpu_are_refused():
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
+    from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
+    x, w = torch.randn(4, 256), torch.ones(256)
+    for call in (lambda: rms_norm(x, w), lambda: rms_norm(x.requires_grad_(True), w), lambda: rms_norm_fp8(x.detach(), w), lambda: route(x, 4),
+                 lambda: balance_loss(x, torch.zeros(4, 2, dtype=torch.int64)), lambda: rms_norm(x.to("meta"), w.to("meta"))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_unknown_scores_are_refused():
+    from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
+    for call in (lambda: route(torch.randn(2, 8), 2, score="relu"), lambda: balance_loss(torch.randn(2, 8), torch.zeros(2, 2, dtype=torch.int64), score="")):
+        with pytest.raises(ValueError, match="score"):
+            call()
+
+
+def test_cases_fit_what_the_operators_take():
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("operator_cases", Path(__file__).resolve().parent.parent / "perf" / "operators.py")
+    M = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(M)
+    assert M.own is False
+    listed = M.listed()
+    most = max(M.work(c)["bytes"] for c in listed)
+    assert 4 <= len(listed) <= 12 and most >= 16 * min(M.work(c)["bytes"] for c in listed)
+    rng = random.Random(0)
+    for c in listed + [M.draw(rng) for _ in range(3000)]:
+        assert M.work(c)["bytes"] <= most
+        if c["kind"].startswith("norm"):
+            assert 1 <= c["hidden"] <= 32768 and (c["kind"] != "norm_fp8" or c["hidden"] % 128 == 0)
+        elif c["kind"] != "balance_grad":
+            size = c["experts"] // c["groups"]
+            assert size * c["groups"] == c["experts"] <= 1024 and c["topk_groups"] <= c["groups"] and c["topk"] <= size * c["topk_groups"] and size >= c["group_best"]
+        assert c["kind"].startswith("norm") or c["padded"] < c["tokens"] or c["tokens"] == 0
