@@ -5,8 +5,8 @@
 // and stays in registers; a warp has a row of up to 128 vectors of 16 bytes, a CTA a longer one; CTAs are persistent, keep
 // their columns' weights in registers and have the next rows under way while they are at one: every thread copies the
 // vectors that it will need itself (cp.async), so that no barrier goes with them. One B200: 8191 x 7168 with a residual to fp8
-// and bf16 90.4 us (5.9 TB/s, 90 % of a copy's rate; without the rows to come under way 97), 16384 x 7168 to bf16 154 to 166,
-// 4095 x 4096 20.2; f16 rows of 1407 (12001 of them) 18.9, bound by instructions, of 1408 14.5; 7 x 7168 3.4.
+// and bf16 91.7 us (5.8 TB/s, 88 % of a copy's rate; without the rows to come under way 97), 16384 x 7168 to bf16 154 to 166,
+// 4095 x 4096 20.2; f16 rows of 1407 (12001 of them) 18.1, bound by instructions, of 1408 14.4; 7 x 7168 3.4.
 #include <cuda_fp8.h>
 #include "../ep/cast.cuh"
 #include "norm.cuh"
