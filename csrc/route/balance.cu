@@ -7,7 +7,7 @@
 // With the counts known the loss is a sum over tokens of F_t, so that the logits are read once forward and once backward:
 // a launch that counts the choices (whole numbers: any order gives the same), one that sums F_t (in 64 bits, in a fixed
 // order). A warp has a run of neighbouring rows and keeps f of their sequence in registers. Bound: latency, of launches for
-// few tokens and of the reductions over a row for many: 16384 x 64 in softmax take 3.0 + 8.9 us forward and 7.5 backward on
+// few tokens and of the reductions over a row for many: 16384 x 64 in softmax take 3.0 + 8.9 us forward and 8.2 backward on
 // one B200, where the logits' bytes would take 0.6 each time.
 #include "route.cuh"
 
@@ -106,8 +106,10 @@ struct Row {
   float p[VPL];              // share of the scores
   float s[VPL];              // sigmoid: 1 - score
   float lse, F;
+  float rest;                // what the shares' sum lacks to 1
   // false: the row takes no part
-  __device__ __forceinline__ bool of(const BalanceParams& a, const Raw<L, VPL>& raw, const float* f) {
+  template <typename V>
+  __device__ __forceinline__ bool of(const BalanceParams& a, const Raw<L, VPL>& raw, const V* f) {
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
@@ -137,28 +139,30 @@ struct Row {
       sum = warp_sum(sum);
     }
     const float inv = 1.f / (sum + kSumEps);
+    rest = kSumEps * inv;
     F = 0.f;
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) { p[k] *= inv; F = fmaf(f[k], p[k], F); }
+    for (int k = 0; k < VPL; ++k) { p[k] *= inv; F = fmaf((float)f[k], p[k], F); }
     F = warp_sum(F);
     return true;
   }
 };
 
 // Rows of a warp, a run of neighbours; f of the sequence that they are in is kept in registers.
-template <int VPL>
+template <int VPL, typename V>
 struct Walk {
   int b = -1;
-  float f[VPL], share = 0.f;
+  V f[VPL];
+  float share = 0.f;
   __device__ __forceinline__ bool to(const BalanceParams& a, long long t, float per_sequence, int lane) {
     const int now = sequence_of(a.seq_off, a.B, t);
     if (now < 0) return false;
     if (now == b) return true;
     b = now;
     const int n = max(1, a.counts[(long long)a.B * a.E + b]);
-    const float unit = (float)a.E / ((float)a.K * (float)n);
+    const V unit = (V)a.E / ((V)a.K * (V)n);
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) f[k] = k * 32 + lane < a.E ? (float)a.counts[(long long)b * a.E + k * 32 + lane] * unit : 0.f;
+    for (int k = 0; k < VPL; ++k) f[k] = k * 32 + lane < a.E ? (V)a.counts[(long long)b * a.E + k * 32 + lane] * unit : (V)0;
     share = per_sequence / (float)n;
     return true;
   }
@@ -176,7 +180,7 @@ balance_loss_kernel(const BalanceParams p, int rows_per_warp) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float per_sequence = sequence_share(p);
   const long long lo = ((long long)blockIdx.x * kBalanceWarps + warp) * rows_per_warp, hi = min(lo + rows_per_warp, (long long)p.T);
-  Walk<VPL> at;
+  Walk<VPL, float> at;
   Raw<L, VPL> raw, next;
   Row<L, VPL> row;
   double mine = 0.0;
@@ -222,7 +226,7 @@ balance_bwd_kernel(const BalanceBwdParams a, int rows_per_warp) {
   const float per_sequence = sequence_share(p);
   const float g = *a.dloss;
   const long long lo = ((long long)blockIdx.x * kBalanceWarps + warp) * rows_per_warp, hi = min(lo + rows_per_warp, (long long)p.T);
-  Walk<VPL> at;
+  Walk<VPL, double> at;
   Raw<L, VPL> raw, next;
   Row<L, VPL> row;
   if (lo < hi) next.load(p, lo, lane);
@@ -231,13 +235,22 @@ balance_bwd_kernel(const BalanceBwdParams a, int rows_per_warp) {
     if (t + 1 < hi) next.load(p, t + 1, lane);
     L* out = static_cast<L*>(a.dlogits) + t * p.E;
     const bool in = at.to(p, t, per_sequence, lane) && row.of(p, raw, at.f);
+    // f - F, where the load is nearly balanced, is a small difference of numbers near each other, and F is off by roundings of
+    // its own size: the difference is taken in 64 bits, and what F is off by, the weighted mean of the differences, out of it
+    float diff[VPL], off = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+      diff[k] = in ? (float)(at.f[k] - (double)row.F) : 0.f;
+      off = fmaf(diff[k], in ? row.p[k] : 0.f, off);
+    }
+    off = warp_sum(off) - (in ? row.F * row.rest : 0.f);
     const float c = g * at.share * p.coeff, z = 2.f * g * at.share * p.z_coeff * (in ? row.lse : 0.f);
 #pragma unroll
     for (int k = 0; k < VPL; ++k) {
       if (k * 32 + lane >= p.E) continue;
       float d = 0.f;
       if (in) {
-        d = c * (at.f[k] - row.F);
+        d = c * (diff[k] - off);
         if (p.score == SCORE_SIGMOID) d *= row.s[k];
         d = row.p[k] * (d + z);
       }

@@ -414,6 +414,32 @@ def test_balance_loss_of_a_perfect_choice_is_its_coefficient():
         assert balance_loss(l, idx, score=score, coeff=0.75).item() == 0.75
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_balance_gradient_of_a_nearly_balanced_choice(score):
+    """f_e - F_t is some 1e-3 of f here; the gradient is as exact as the shares that it multiplies."""
+    from gpu_data_transfer_profile_b200.ops.router import balance_loss
+    T, E, K = 4096, 64, 4
+    idx = (torch.arange(T, device="cuda")[:, None] * K + torch.arange(K, device="cuda")) % E
+    idx[5, 0], idx[100, 1], idx[101, 2] = 9, 9, 40
+    l = torch.randn(T, E, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    a, wide = l.clone().requires_grad_(True), l.double().requires_grad_(True)
+    got, = torch.autograd.grad(balance_loss(a, idx, score=score), a)
+    ref, = torch.autograd.grad(_balance(wide, idx, score, 1.0, 0.0, None), wide)
+    # shares off by some 2^-22, their weighted sum by the mean of 64 of those: relative to the gradient itself
+    assert (got.double() - ref).norm() <= ref.norm() * 1e-6
+    even = torch.autograd.grad(balance_loss(a, (torch.arange(T, device="cuda")[:, None] * K + torch.arange(K, device="cuda")) % E, score=score), a)[0]
+    # (all f are 1; F is off by 2^-22 and its correction by as much of that)
+    assert even.abs().max() <= 2.0 ** -43
+    # the other extreme: one expert has all choices, and the smallest share of the tokens' scores by far
+    l = torch.randn(50, 3, device="cuda") - torch.tensor([12.0, 0.0, 0.0], device="cuda")
+    a, wide = l.clone().requires_grad_(True), l.double().requires_grad_(True)
+    idx = torch.zeros(50, 1, dtype=torch.int64, device="cuda")
+    loss, want = balance_loss(a, idx, score=score), _balance(wide, idx, score, 1.0, 0.0, None)
+    assert abs(loss.item() / want.item() - 1) < 1e-6
+    got, ref = torch.autograd.grad(loss, a)[0], torch.autograd.grad(want, wide)[0]
+    assert (got.double() - ref).norm() <= ref.norm() * 1e-6
+
+
 def test_balance_loss_strides_empty_and_unused():
     from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
     big = torch.randn(50, 200, device="cuda")
