@@ -6,7 +6,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-V3 = dict(score="sigmoid", num_groups=4, topk_groups=2, group_best=2, renormalize=True, route_scale=2.5, expert_bias=True)
+GROUPED = dict(score="sigmoid", num_groups=4, topk_groups=2, group_best=2, renormalize=True, route_scale=2.5, expert_bias=True)
 
 
 @pytest.fixture
@@ -85,7 +85,7 @@ def _reference(layer, x, logits, residual, off):
 
 @pytest.mark.parametrize("mode", ["fused", "deepep"])
 @pytest.mark.parametrize("kw", [
-    dict(norm=True, balance_coeff=0.5, **V3),
+    dict(norm=True, balance_coeff=0.5, **GROUPED),
     dict(norm=True, balance_coeff=0.5, z_coeff=0.01, renormalize=False),
     dict(score="sigmoid", balance_coeff=1.0), dict(num_groups=4, topk_groups=2), dict(norm=True)])
 def test_training_step_against_every_step_written_out(world, kw, mode):
@@ -116,7 +116,7 @@ def test_training_step_against_every_step_written_out(world, kw, mode):
         torch.testing.assert_close(a, b, atol=2e-4 * max(1.0, b.abs().max().item()), rtol=2e-3)
 
 
-@pytest.mark.parametrize("kw", [dict(norm=True, **V3), dict(V3), dict(norm=True, score="softmax", renormalize=False, num_groups=4, topk_groups=1), dict(norm=True)])
+@pytest.mark.parametrize("kw", [dict(norm=True, **GROUPED), dict(GROUPED), dict(norm=True, score="softmax", renormalize=False, num_groups=4, topk_groups=1), dict(norm=True)])
 @pytest.mark.parametrize("fuse", [True, False])
 def test_inference_against_every_step_written_out(world, kw, fuse):
     """bf16, tensor-core experts, rows consumed in place; the same layer with gradients goes the general way."""
@@ -144,7 +144,7 @@ def test_inference_against_every_step_written_out(world, kw, fuse):
 @pytest.mark.parametrize("fuse", [True, False])
 @pytest.mark.parametrize("none", [False, True])
 def test_padding_rows_reach_no_expert(world, grad, fuse, none):
-    layer = _layer(world, fuse_combine=fuse, balance_coeff=1.0, **V3)
+    layer = _layer(world, fuse_combine=fuse, balance_coeff=1.0, **GROUPED)
     T, E = 100, 16
     x = torch.randn(T, 256, device="cuda").to(torch.bfloat16).requires_grad_(grad)
     logits = torch.randn(T, E, device="cuda")
@@ -172,7 +172,7 @@ def test_padding_rows_reach_no_expert(world, grad, fuse, none):
 @pytest.mark.parametrize("T", [1, 37, 200])
 def test_fp8_rows_of_the_norm_go_straight_into_the_exchange(world, T, monkeypatch):
     from gpu_data_transfer_profile_b200.models import moe_layer as M
-    layer = _layer(world, use_fp8=True, norm=True, **V3)
+    layer = _layer(world, use_fp8=True, norm=True, **GROUPED)
     x, r = (torch.randn(T, 256, device="cuda").to(torch.bfloat16) for _ in range(2))
     calls = []
     real = M.N.rms_norm_fp8
@@ -201,7 +201,7 @@ def test_router_logits_kernel_against_64_bits():
 
 def test_replaced_routers_and_refusals(world, monkeypatch):
     from gpu_data_transfer_profile_b200.models import moe_layer as M
-    layer = _layer(world, **V3)
+    layer = _layer(world, **GROUPED)
     x = torch.randn(20, 256, device="cuda").to(torch.bfloat16)
     fixed = torch.arange(4, device="cuda").expand(20, 4).contiguous()
     with torch.no_grad():
@@ -219,4 +219,4 @@ def test_replaced_routers_and_refusals(world, monkeypatch):
 def test_state_of_a_default_layer_is_what_it_was(world):
     layer = _layer(world)
     assert sorted(layer.state_dict()) == ["experts.weight1", "experts.weight2", "router.weight"]
-    assert sorted(_layer(world, norm=True, **V3).state_dict()) == ["expert_bias", "experts.weight1", "experts.weight2", "norm_weight", "router.weight"]
+    assert sorted(_layer(world, norm=True, **GROUPED).state_dict()) == ["expert_bias", "experts.weight1", "experts.weight2", "norm_weight", "router.weight"]
