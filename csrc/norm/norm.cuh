@@ -224,6 +224,12 @@ __device__ __forceinline__ float inverse_root(float v) {
   const float r = rsqrtf(v);
   return v > 0.f && v < INFINITY ? fmaf(r * 0.5f, fmaf(-(v * r), r, 1.f), r) : r;
 }
+// 1 / v for v > 0 likewise, without the branches of a division; 0 for infinity.
+__device__ __forceinline__ float inverse(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return v < INFINITY ? fmaf(r, fmaf(-v, r, 1.f), r) : r;
+}
 
 // After how many rows the place of a row's first element within 16 bytes comes again.
 inline int align_period(long long ld_bytes) {

@@ -5,7 +5,7 @@
 // and stays in registers; a warp has a row of up to 128 vectors of 16 bytes, a CTA a longer one; CTAs are persistent, keep
 // their columns' weights in registers and have the next rows under way while they are at one: every thread copies the
 // vectors that it will need itself (cp.async), so that no barrier goes with them. One B200: 8191 x 7168 with a residual to fp8
-// and bf16 91.7 us (5.8 TB/s, 88 % of a copy's rate; without the rows to come under way 97), 16384 x 7168 to bf16 154 to 166,
+// and bf16 88.6 us (6.0 TB/s, 92 % of a copy's rate; without the rows to come under way 97), 16384 x 7168 to bf16 154 to 166,
 // 4095 x 4096 20.2; f16 rows of 1407 (12001 of them) 18.1, bound by instructions, of 1408 14.4; 7 x 7168 3.4.
 #include <cuda_fp8.h>
 #include "../ep/cast.cuh"
@@ -119,7 +119,7 @@ rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
 #pragma unroll
         for (int o = kNormScaleBlock / EPV / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         amax = fmaxf(amax, 1e-4f);
-        const float2 inv = both(448.f / amax);
+        const float2 inv = both(448.f * inverse(amax));
         if (e0 < H) {
           uint32_t o[EPV / 4];
 #pragma unroll
@@ -160,9 +160,10 @@ int launch_fwd_sized(const NormFwdParams& p, cudaStream_t st) {
   if (nvec <= 64) return launch_fwd<T, W, 2, FP8, true, ALIGNED>(p, kWarpRows * 32, st);
   if (nvec <= 128) return launch_fwd<T, W, 4, FP8, true, ALIGNED>(p, kWarpRows * 32, st);
   const auto threads = [nvec](int vpt) { return ((nvec + vpt - 1) / vpt + 31) / 32 * 32; };
-  // The cast to 8 bits wants more warps (8191 x 7168: 95.7 us with two vectors a thread, 90.2 with one), without it fewer
-  // and longer threads are as good or better (12001 x 1408 in f16: 14.6 and 16.7).
-  if (FP8 && nvec > 256 && nvec <= 1024) return launch_fwd<T, W, 1, FP8, false, ALIGNED>(p, threads(1), st);
+  // The cast of 16-bit rows wants more warps (8191 x 7168: 95.7 us with two vectors a thread, 90.2 with one), without it, and
+  // of f32 rows, fewer and longer threads are as good or better (12001 x 1408 in f16: 14.6 and 16.7; 8191 x 4096 in f32 to
+  // fp8: 52.0 and 68.8).
+  if (FP8 && sizeof(T) == 2 && nvec > 256 && nvec <= 1024) return launch_fwd<T, W, 1, FP8, false, ALIGNED>(p, threads(1), st);
   if (nvec <= 2048) return launch_fwd<T, W, 2, FP8, false, ALIGNED>(p, threads(2), st);
   if (nvec <= 4096) return launch_fwd<T, W, 4, FP8, false, ALIGNED>(p, threads(4), st);
   return launch_fwd<T, W, 9, FP8, false, ALIGNED>(p, threads(9), st);
