@@ -12,10 +12,6 @@ namespace norm {
 
 template <typename T> constexpr int kEpv = 16 / (int)sizeof(T);      // elements of a vector
 
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f(float v) { return v; }
-template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }

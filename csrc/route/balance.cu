@@ -14,16 +14,16 @@
 namespace b200ep {
 namespace route {
 
-// The sequence that row t belongs to, -1 for none: the last one that begins at or before it, if it ends behind it.
+// The sequence that row t belongs to, -1 for none: of those that begin at or before it the last.
 __device__ __forceinline__ int sequence_of(const int* off, int B, long long t) {
   if (off == nullptr) return 0;
-  int lo = 0, hi = B;                                       // off[lo] <= t < off[hi], if at all
   if (t < (long long)__ldg(off) || t >= (long long)__ldg(off + B)) return -1;
+  int lo = 0, hi = B;                                       // off[lo] <= t < off[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if ((long long)__ldg(off + mid) <= t) lo = mid; else hi = mid;
   }
-  return t < (long long)__ldg(off + lo + 1) ? lo : -1;
+  return lo;
 }
 
 // Choices and rows with a choice, counted in shared memory for a run of rows of one sequence at a time.
@@ -38,37 +38,33 @@ balance_count_kernel(const BalanceParams p, int rows_per) {
   const uint32_t one_row = K == 32 ? 0xffffffffu : (1u << K) - 1;
   const long long lo = (long long)blockIdx.x * rows_per, hi = min(lo + rows_per, (long long)p.T);
   for (long long at = lo; at < hi;) {
-    if (p.seq_off != nullptr) {                             // (rows outside all sequences at either end are passed over at once)
-      if (at >= (long long)__ldg(p.seq_off + p.B)) break;
-      if (at < (long long)__ldg(p.seq_off)) { at = (long long)__ldg(p.seq_off); continue; }
-    }
-    const int b = sequence_of(p.seq_off, p.B, at);
     long long end = hi;
+    int b = 0;
     if (p.seq_off != nullptr) {
-      if (b >= 0) end = min(end, (long long)__ldg(p.seq_off + b + 1));
-      else end = at + 1;                                    // (outside every sequence: look at the next row)
+      if (at >= (long long)__ldg(p.seq_off + p.B)) break;   // (rows outside all sequences are passed over)
+      if (at < (long long)__ldg(p.seq_off)) { at = (long long)__ldg(p.seq_off); continue; }
+      b = sequence_of(p.seq_off, p.B, at);
+      end = min(end, (long long)__ldg(p.seq_off + b + 1));
     }
-    if (b >= 0) {
-      for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
-      if (threadIdx.x == 0) s_rows = 0;
-      __syncthreads();
-      int live = 0;
-      for (long long t0 = at + warp * rows_at_once; t0 < end; t0 += (long long)(blockDim.x >> 5) * rows_at_once) {
-        const long long t = t0 + sub;
-        const long long i = sub < rows_at_once && t < end ? __ldg(p.idx + t * K + choice) : -1;
-        const bool ok = i >= 0 && i < E;
-        if (ok) atomicAdd(s_count + (int)i, 1);
-        const uint32_t some = __ballot_sync(0xffffffffu, ok);
-        if (choice == 0 && sub < rows_at_once && (some >> (sub * K) & one_row)) ++live;
-      }
-      live = __reduce_add_sync(0xffffffffu, live);
-      if (lane == 0 && live) atomicAdd(&s_rows, live);
-      __syncthreads();
-      for (int e = threadIdx.x; e < E; e += blockDim.x)
-        if (s_count[e]) atomicAdd(p.counts + (long long)b * E + e, s_count[e]);
-      if (threadIdx.x == 0 && s_rows) atomicAdd(p.counts + (long long)p.B * E + b, s_rows);
-      __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
+    if (threadIdx.x == 0) s_rows = 0;
+    __syncthreads();
+    int live = 0;
+    for (long long t0 = at + warp * rows_at_once; t0 < end; t0 += (long long)(blockDim.x >> 5) * rows_at_once) {
+      const long long t = t0 + sub;
+      const long long i = sub < rows_at_once && t < end ? __ldg(p.idx + t * K + choice) : -1;
+      const bool ok = i >= 0 && i < E;
+      if (ok) atomicAdd(s_count + (int)i, 1);
+      const uint32_t some = __ballot_sync(0xffffffffu, ok);
+      if (choice == 0 && sub < rows_at_once && (some >> (sub * K) & one_row)) ++live;
     }
+    live = __reduce_add_sync(0xffffffffu, live);
+    if (lane == 0 && live) atomicAdd(&s_rows, live);
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x)
+      if (s_count[e]) atomicAdd(p.counts + (long long)b * E + e, s_count[e]);
+    if (threadIdx.x == 0 && s_rows) atomicAdd(p.counts + (long long)p.B * E + b, s_rows);
+    __syncthreads();
     at = end;
   }
 }
