@@ -2,6 +2,7 @@
 // Raw addresses cross the boundary as int64; tensors are checked for device/dtype here.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <chrono>

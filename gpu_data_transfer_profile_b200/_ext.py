@@ -99,6 +99,8 @@ def _import_so():
 def load():
     """Return the native module, building it when missing or stale."""
     global _mod
+    if _mod is not None:                 # (complete as soon as it is set; every call of an operator comes by here)
+        return _mod
     with _lock:
         if _mod is None:
             if is_built():
