@@ -8,6 +8,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+U_F32 = 2.0 ** -24
 
 
 def _half(dt):
@@ -226,6 +227,23 @@ def test_fp8(H, dt):
             _close(y, want, dt)                                    # (rms_norm's may be another of two neighbours: other lanes sum the squares)
         if residual:
             _close(h, hw, dt)
+
+
+def test_more_dimensions_and_a_tensor_given_twice():
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
+    x, r, w = _inputs((2, 3, 5, 384), BF16, F32, True)
+    (q, s), y, h = rms_norm_fp8(x, w, residual=r, keep=True)
+    (q2, s2), y2, h2 = rms_norm_fp8(x.view(30, 384), w, residual=r.view(30, 384), keep=True)
+    assert q.shape == x.shape and s.shape == (2, 3, 5, 3) and torch.equal(q.view(torch.uint8).view(30, 384), q2.view(torch.uint8))
+    assert torch.equal(s.view(30, 3), s2) and torch.equal(y.view(30, 384), y2) and torch.equal(h.view(30, 384), h2)
+    a = torch.randn(4, 6, 100, device="cuda").transpose(0, 1).requires_grad_(True)
+    wide = a.detach().double().requires_grad_(True)
+    w = torch.ones(100, device="cuda")
+    y, h = rms_norm(a, w, residual=a)
+    yw, hw = _wide(wide, w, wide, 1e-6)
+    got, ref = torch.autograd.grad((y * y * h).sum(), a)[0], torch.autograd.grad((yw * yw * hw).sum(), wide)[0]
+    # products of three numbers below 10 and a mean of 100 of them: 32-bit roundings of some hundreds
+    assert got.shape == a.shape and ((got.double() - ref).abs() <= 1000 * 100 * U_F32).all()
 
 
 def test_fp8_rows_feed_the_grouped_gemm():
