@@ -562,7 +562,8 @@ __device__ __forceinline__ void store_choice(const RouteParams& p, const L* row,
     p.w[t * p.K + k] = e < 0 ? 0.f : (p.renorm ? s * reciprocal(chosen + kSumEps) : s) * p.scale;
     if (p.aux != nullptr && !soft) p.aux[t * p.K + k] = l;
   }
-  if (p.aux != nullptr && soft && !p.renorm && k < 2) p.aux[t * 2 + k] = k == 0 ? top : (sum > 0.f || sum != sum ? 1.f / sum : 0.f);
+  if (p.aux != nullptr && soft && k < 3)
+    p.aux[t * 3 + k] = k == 0 ? top : k == 1 ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : kSumEps * reciprocal(chosen + kSumEps);
 }
 
 template <typename L, int VPL, int MODE>
@@ -583,10 +584,15 @@ route_kernel(const __grid_constant__ RouteParams p, const __grid_constant__ Grou
 // Gradient of the logits, a warp per token. With g the weights' gradient times `scale`:
 //   sigmoid:                d l_k = s_k (1 - s_k) h_k for the choices, 0 for the others; h = g, or renormalised
 //                           h_k = (g_k - sum_j g_j s_j / S) / S with S = sum_j s_j + 1e-20
-//   softmax, renormalised:  the weights are a softmax over the chosen logits: d l_k = u_k (g_k - sum_j u_j g_j), u = w / scale
 //   softmax as it is:       d l_e = p_e ([e chosen] g_e - sum_j g_j p_j) for every expert
-// Bound: memory, the zeros written to [T, E] above all; only the last form reads the logits again. 16384 x 256 in f32: 6.3 us
-// (2.7 TB/s).
+//   softmax, renormalised:  with u = w / scale, D = sum_j u_j g_j and r = 1e-20 / S, which is 1 - sum_j u_j,
+//                           d l_e = [e chosen] u_e (g_e - D) - p_e r D for every expert
+// r is kept by the forward: 1 less the sum of the u would be their roundings. It is next to nothing (the weights are a softmax over
+// the chosen logits) unless an expert that a bias or its group keeps out of the choice lies far above those in it: from 46
+// on, r is a half or more. g_e - D is taken as (g_e sum_j u_j - D) + r g_e, whose first part is 0 where there is one choice.
+// Bound: memory, the zeros written to [T, E] above all; the logits are read again by softmax as it is, and for rows whose r
+// tells. 16384 x 256 in f32: 6.3 us (2.7 TB/s).
+constexpr float kLackTells = 0x1p-40f;   // r below this (S above 1.1e-8) changes no gradient by more than 2^-40 of the g
 template <typename L>
 __global__ void __launch_bounds__(256)
 route_bwd_kernel(const RouteBwdParams p) {
@@ -619,14 +625,20 @@ route_bwd_kernel(const RouteBwdParams p) {
   } else {
     const float u = e >= 0 ? p.w[t * p.K + lane] / p.scale : 0.f;
     const float dot = warp_sum(u * g);
-    // (renormalised, their sum is 1 but for roundings, which g times the sum takes out: no gradient where there is one choice)
-    d = u * ((p.renorm ? g * warp_sum(u) : g) - dot);
-    if (!p.renorm) {
+    float rest = dot;                                       // what every expert's gradient has, times -p_e
+    d = u * (g - dot);
+    if (p.renorm) {
+      const float lack = p.aux[t * 3 + 2];
+      const bool tells = lack > kLackTells;
+      rest = tells ? lack * dot : 0.f;
+      d = u * ((__fmul_rn(g, warp_sum(u)) - dot) + (tells ? lack * g : 0.f));
+    }
+    if (rest != 0.f) {
       const L* row = static_cast<const L*>(p.logits) + t * p.ld;
-      const float top = p.aux[t * 2], inv = p.aux[t * 2 + 1];
-      for (int j = lane; j < E; j += 32) put(out + j, expf(logit(row + j) - top) * inv * -dot);
+      const float top = p.aux[t * 3], inv = p.aux[t * 3 + 1];
+      for (int j = lane; j < E; j += 32) put(out + j, expf(logit(row + j) - top) * inv * -rest);
       __syncwarp();
-      if (e >= 0) put(out + e, d);
+      if (e >= 0) put(out + e, p.renorm ? fmaf(expf(logit(row + e) - top) * inv, -rest, d) : d);
       return;
     }
   }

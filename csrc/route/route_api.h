@@ -23,14 +23,14 @@ struct RouteParams {
   float scale;               // > 0
   long long* idx;            // [T, K]
   float* w;                  // f32 [T, K]
-  float* aux;                // for the backward, or null: sigmoid the chosen logits [T, K], softmax without renormalising
-                             // {maximum, 1 / sum} [T, 2], otherwise nothing
+  float* aux;                // for the backward, or null: sigmoid the chosen logits [T, K], softmax {maximum, 1 / sum, what
+                             // the renormalised weights lack to a sum of 1} [T, 3]
 };
 int launch_route(const RouteParams& p, cudaStream_t st);
 
 struct RouteBwdParams {
   int type;
-  const void* logits;        // read by softmax without renormalising only
+  const void* logits;        // read by softmax only
   long long ld;
   int T, E, K, score;
   bool renorm;

@@ -263,6 +263,43 @@ def test_route_gradient_of_one_renormalised_choice_is_zero():
     assert (torch.autograd.grad(w, l, torch.randn(500, 1, device="cuda"))[0] == 0).all()
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("bar", [-math.inf, -2.0])
+@pytest.mark.parametrize("K", [1, 3])
+@pytest.mark.parametrize("gap", [10, 20, 30, 40, 46, 60])
+def test_route_gradient_where_the_favourite_may_not_be_chosen(gap, K, bar, dt):
+    """The chosen scores sum to little beside the 1e-20 that is added: the weights are no softmax over the chosen logits."""
+    from gpu_data_transfer_profile_b200.ops.router import route
+    g = torch.Generator(device="cuda").manual_seed(gap + K)
+    T, E, scale = 40, 41, 2.5
+    l = torch.randn(T, E, generator=g, device="cuda") * 1.5
+    bias = torch.zeros(E, device="cuda")
+    bias[7] = bar
+    l[:, 7] = l.max(1).values + gap
+    l[3] = -math.inf                                                # padding
+    l = l.to(dt).requires_grad_(True)
+    idx, w = route(l, K, bias=bias, scale=scale)
+    dw = torch.randn(T, K, generator=g, device="cuda")
+    got, = torch.autograd.grad(w, l, dw)
+    lw = l.detach().double().requires_grad_(True)
+    want = _weights(lw, idx, "softmax", True, scale)
+    ref, = torch.autograd.grad(want, lw, dw.double())
+    ref = torch.where(torch.isneginf(l), 0.0, ref)
+    assert not (idx == 7).any() and (idx[3] == -1).all() and (got[3] == 0).all()
+    # Distances of up to 70 to the maximum are rounded by 64 U, so is each score relative to itself. A weight has two of them,
+    # two sums of up to 41 and 3 + K roundings, what it is multiplied by as many again: below 800 U of the terms' sizes. Of
+    # one choice, the first term's difference is 0. Below 2^-40 the lack is left out.
+    p = torch.softmax(torch.where(torch.isneginf(lw), -1e4, lw), 1).detach()
+    u = want.detach() / scale
+    r = 1e-20 / (p.gather(1, idx.clamp_min(0)).sum(1, keepdim=True) + 1e-20)
+    dg = dw.double().abs() * scale
+    all_g = (u * dg).sum(1, keepdim=True)
+    tol = (800 * U * r + 2.0 ** -40) * p * all_g
+    tol = tol.scatter_add(1, idx.clamp_min(0), (800 * U * r + 2.0 ** -40) * u * dg + (0 if K == 1 else 800 * U * u * (dg + all_g)))
+    tol = tol + ref.abs() * (torch.finfo(dt).eps / 2 * 1.01 if dt != F32 else 0) + (2.0 ** -25 if dt == F16 else 0)
+    assert ((got.double() - ref).abs() <= tol).all()
+
+
 def test_route_gradient_against_differences():
     from gpu_data_transfer_profile_b200.ops.router import route
     g = torch.Generator(device="cuda").manual_seed(0)
@@ -281,6 +318,28 @@ def test_route_gradient_against_differences():
         want = ((wp - wm).double() * dw).sum(1) / (2 * s)
         # third derivatives below 20 a token times s^2 / 6; roundings of the weights over 2 s
         assert ((got - want).abs()[same] < 20 * 3 * s * s + 4 * 3 * 4 * 8 * U / s).all()
+
+
+def test_route_gradient_against_differences_where_the_favourite_may_not_be_chosen():
+    from gpu_data_transfer_profile_b200.ops.router import route
+    g = torch.Generator(device="cuda").manual_seed(5)
+    l = torch.randn(40, 24, generator=g, device="cuda")
+    l[:, 9] = 46.0                                                  # 1e-20 of it and the chosen scores are of one size
+    bias = torch.zeros(24, device="cuda")
+    bias[9] = -math.inf
+    u = torch.randn(40, 24, generator=g, device="cuda").clamp(-1, 1)
+    dw = torch.randn(40, 4, generator=g, device="cuda").clamp(-2, 2)
+    a = l.clone().requires_grad_(True)
+    idx, w = route(a, 4, bias=bias)
+    got = (torch.autograd.grad(w, a, dw)[0] * u).sum(1).double()
+    s = 2.0 ** -6
+    (ip, wp), (im, wm) = (route(l + d * u, 4, bias=bias) for d in (s, -s))
+    same = ((ip == idx) & (im == idx)).all(1)
+    assert same.sum() > 20 and got.abs().max() > 0.1
+    want = ((wp - wm).double() * dw).sum(1) / (2 * s)
+    # (third derivatives below 50: of a softmax along directions of up to 2 with a gradient of up to 2 each; scores rounded by
+    # 32 U for their distance of 46 to the maximum, weights by three times that)
+    assert ((got - want).abs()[same] < 50 * s * s / 6 + 4 * 2 * 100 * U / s).all()
 
 
 def test_route_refusals():
