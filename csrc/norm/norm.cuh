@@ -220,7 +220,7 @@ __device__ __forceinline__ float inverse_root(float v) {
   const float r = rsqrtf(v);
   return v > 0.f && v < INFINITY ? fmaf(r * 0.5f, fmaf(-(v * r), r, 1.f), r) : r;
 }
-// 1 / v for v > 0 likewise, without the branches of a division; 0 for infinity.
+// 1 / v for 2^-126 <= v <= 2^126 likewise, without the branches of a division; 0 above (the approximation has no denormals).
 __device__ __forceinline__ float inverse(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

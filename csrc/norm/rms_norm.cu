@@ -119,7 +119,7 @@ rms_norm_fwd_kernel(const __grid_constant__ NormFwdParams p, int stages) {
 #pragma unroll
         for (int o = kNormScaleBlock / EPV / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         amax = fmaxf(amax, 1e-4f);
-        const float2 inv = both(448.f * inverse(amax));
+        const float2 inv = both(1.75f * inverse(amax * 0x1p-8f));      // 448 / amax (a power of 2 aside, so that every finite amax has one)
         if (e0 < H) {
           uint32_t o[EPV / 4];
 #pragma unroll

@@ -33,6 +33,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[to
     """-> ((q e4m3 [..., H], scales f32 [..., H/128]), y, h): what `Buffer.dispatch` takes in place of rows and
     `ops.gemm.grouped_gemm_fp8` multiplies; scale = max(amax, 1e-4) / 448 of 128 channels of y, as in the cast of an fp8
     dispatch, here of y before its rounding. y in the type of x if `keep` (for a router beside the experts), else None; h is
-    None without a residual. H is a multiple of 128. For inference: refuses inputs that require a gradient."""
+    None without a residual. H is a multiple of 128. NaN stays NaN in q and takes no part in its block's scale; a block with
+    an infinite y has an infinite scale. For inference: refuses inputs that require a gradient."""
     q, scales, y, h = _ext.load().rms_norm_fp8(x, weight, residual, eps, keep)
     return (q, scales), y, h

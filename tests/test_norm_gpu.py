@@ -229,6 +229,50 @@ def test_fp8(H, dt):
             _close(h, hw, dt)
 
 
+@pytest.mark.parametrize("dt,wdt", [(BF16, BF16), (BF16, F32), (F32, F32)])
+@pytest.mark.parametrize("size", [1e-36, 4e35, 5e37])
+def test_fp8_of_very_small_and_very_large_weights(size, dt, wdt):
+    """Blocks whose largest value lies above 2^126 (8.5e37) and near the largest number of 32 bits."""
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm_fp8
+    x, _, w = _inputs((60, 512), dt, wdt, False, seed=3)
+    w = (w.float() * size).to(wdt)
+    x[5, 7] = 100.0                                                # 16 times the others: up to 3e38
+    (q, s), y, _ = rms_norm_fp8(x, w, keep=True)
+    want, _ = _wide(x, w, None, 1e-6)
+    blocks = want.view(60, 4, 128)
+    amax = blocks.abs().amax(-1)
+    fits = amax < torch.finfo(F32).max * (1 - 50 * _half(F32))      # (the others are infinite in 32 bits, and so are their scales)
+    assert fits.float().mean() > 0.9 and (size < 1e37 or (amax[fits] > 1.5e38).any())
+    scale = amax.clamp_min(1e-4) / 448
+    torch.testing.assert_close(s.double()[fits], scale[fits], atol=0, rtol=50 * _half(F32))
+    assert (s[amax > torch.finfo(F32).max * (1 + 50 * _half(F32))] == math.inf).all()
+    got = q.float().double().view_as(blocks) * s.double()[..., None]
+    tol = blocks.abs() * (2.0 ** -4 + 120 * _half(F32)) + scale[..., None] * 2.0 ** -10 * 1.001
+    assert ((got - blocks).abs() <= tol)[fits].all()
+
+
+def test_fp8_of_infinities_and_nan():
+    """What is not a number stays that, and takes no part in its block's scale; an infinite block has an infinite scale."""
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm_fp8
+    x = torch.randn(4, 256, device="cuda")
+    w = torch.ones(256, device="cuda")
+    x[1, 3] = math.nan                                             # the row's root is none
+    x[2, 130] = math.inf                                           # the row's root is 0: the others become 0
+    (q, s), y, _ = rms_norm_fp8(x, w, keep=True)
+    v = q.float()
+    assert v[1].isnan().all() and (s[1:3] == torch.tensor(1e-4, device="cuda") * (1 / 448)).all()
+    assert v[2, 130].isnan() and (v[2, :130] == 0).all() and (v[2, 131:] == 0).all() and y[2, 130].isnan()
+    clean = rms_norm_fp8(x[[0, 3]], w)[0]
+    assert torch.equal(q[[0, 3]].view(torch.uint8), clean[0].view(torch.uint8)) and torch.equal(s[[0, 3]], clean[1])
+    w[5], w[200] = math.nan, math.inf
+    (q, s), _, _ = rms_norm_fp8(x[:1], w)
+    v = q.float()
+    other = torch.arange(256, device="cuda") != 5
+    want, _ = _wide(x[:1], torch.ones(256, device="cuda"), None, 1e-6)
+    assert v[0, 5].isnan() and v[0, :128][other[:128]].isfinite().all() and s[0, 1] == math.inf
+    torch.testing.assert_close(s[0, 0].double(), want[0, :128][other[:128]].abs().max() / 448, atol=0, rtol=50 * _half(F32))
+
+
 def test_more_dimensions_and_a_tensor_given_twice():
     from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
     x, r, w = _inputs((2, 3, 5, 384), BF16, F32, True)
