@@ -23,7 +23,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.
     """y, or (y, h) with a residual (shape and type of x): h is the residual of the next block.
 
     Differentiable once in x, residual and weight; the weight's gradient is summed in a fixed order. No forward-mode
-    derivatives, no function transforms (refused)."""
+    derivatives, no function transforms, no tracing (refused)."""
     y, h = _ext.load().rms_norm(x, weight, residual, eps)
     return y if residual is None else (y, h)
 

@@ -34,7 +34,7 @@ def route(logits: torch.Tensor, topk: int, *, score: str = "softmax", bias: Opti
 
     An expert whose logit or bias is -inf is not available: where fewer than topk are left, the index is -1 (no expert, to
     every call of this package) and the weight 0, for all choices of a padding row. NaN ranks above everything. topk and
-    num_groups are at most 32. Differentiable once in the logits; no forward-mode derivatives, no function transforms."""
+    num_groups are at most 32. Differentiable once in the logits; no forward-mode derivatives, no function transforms, no tracing (refused)."""
     return _ext.load().route_experts(logits, topk, _score(score), bias, num_groups, num_groups if topk_groups is None else topk_groups,
                                      group_best, renormalize, scale)
 
@@ -49,5 +49,5 @@ def balance_loss(logits: torch.Tensor, idx: torch.Tensor, *, score: str = "softm
     and the mean of that over the sequences that have such tokens; 0 where none has. seq_off (int32 [B + 1], ascending, on
     the logits' device) cuts the rows into B packed sequences; rows outside take no part. Default: one sequence of all rows.
     Differentiable once in the logits (f is a count); rows that take no part get a gradient of 0. No forward-mode
-    derivatives, no function transforms."""
+    derivatives, no function transforms, no tracing (refused)."""
     return _ext.load().balance_loss(logits, idx, seq_off, _score(score), coeff, z_coeff)

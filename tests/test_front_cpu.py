@@ -19,6 +19,28 @@ def test_tensors_on_the_cpu_are_refused():
             call()
 
 
+def _traced():
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
+    from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
+    w, idx = torch.ones(256), torch.zeros(4, 2, dtype=torch.int64)
+    return (lambda x: rms_norm(x, w.to(x.device)), lambda x: rms_norm(x, w.to(x.device), residual=x)[0], lambda x: rms_norm_fp8(x, w.to(x.device))[0][1],
+            lambda x: route(x, 4)[1], lambda x: balance_loss(x, idx.to(x.device)))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_tracing_is_refused(device):
+    """A tracer would keep the example's outputs as constants."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(4, 256, device=device)
+    for call in _traced():
+        with pytest.raises(RuntimeError, match="tracing"):
+            torch.jit.trace(call, (x,))
+        with pytest.raises(RuntimeError, match="tracing"):
+            make_fx(call)(x)
+        if device == "cuda":
+            assert call(x).device == x.device
+
+
 def test_unknown_scores_are_refused():
     from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
     for call in (lambda: route(torch.randn(2, 8), 2, score="relu"), lambda: balance_loss(torch.randn(2, 8), torch.zeros(2, 2, dtype=torch.int64), score="")):
