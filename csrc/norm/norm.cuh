@@ -109,10 +109,11 @@ __device__ __forceinline__ void store_vec(char* at, int e0, int H, const uint4& 
   }
 }
 
-// A row's vector straight from memory, zeros outside the row.
+// A row's vector straight from memory, zeros outside the row. (Coherent loads, as of all inputs: the kernel before, in stream order,
+// may still write what this one reads when its CTAs are placed.)
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ uint4 load_vec(const T* row, int e0, int H) {
-  if (ALIGNED || whole<T>(e0, H)) return ld_global_nc_v4(row + e0);
+  if (ALIGNED || whole<T>(e0, H)) return ld_global_once_v4(row + e0);
   union { uint4 v; T e[kEpv<T>]; } u;
   u.v = make_uint4(0, 0, 0, 0);
 #pragma unroll
@@ -164,7 +165,7 @@ struct WeightVec {
   __device__ __forceinline__ void load(const W* w, int e0, int H, bool aligned) {
     if (aligned && whole<T>(e0, H)) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = ld_global_nc_v4(w + e0 + i * kEpv<W>);
+      for (int i = 0; i < N; ++i) r[i] = ld_global_v4(w + e0 + i * kEpv<W>);
       return;
     }
 #pragma unroll

@@ -74,10 +74,10 @@ rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int stages) {
   uint32_t from = mine;
   const long long out_step = (long long)step * H;
   long long out = (long long)row0 * H;                      // the row in a contiguous tensor
-  float next_rstd = row0 < p.T ? __ldg(p.rstd + row0) : 0.f;
+  float next_rstd = row0 < p.T ? p.rstd[row0] : 0.f;
   for (long long row = row0; row < p.T; row += step, out += out_step, parity ^= 1) {
     const float rstd = next_rstd;
-    if (row + step < p.T) next_rstd = __ldg(p.rstd + row + step);
+    if (row + step < p.T) next_rstd = p.rstd[row + step];
     if constexpr (STAGED) fetch_wait(stages - 1);
     const auto vec = [&](uint32_t at, int i, const void* t, long long ld, int e0) {
       if constexpr (STAGED) return inside<T, ALIGNED>(lds_v4(from + at + i * word), e0);
@@ -180,7 +180,7 @@ rms_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int stages) {
 // dw[e] = sum of the parts: 32 columns a CTA, 32 strands of parts side by side, joined by a tree.
 template <typename W>
 __global__ void __launch_bounds__(1024)
-sum_rows_kernel(const float* __restrict__ part, int parts, int H, W* __restrict__ dw) {
+sum_rows_kernel(const float* part, int parts, int H, W* dw) {
   stream_order_wait();
   stream_order_next();
   __shared__ float s[32][33];
@@ -188,7 +188,7 @@ sum_rows_kernel(const float* __restrict__ part, int parts, int H, W* __restrict_
   float v = 0.f;
   if (e < H) {
 #pragma unroll 8
-    for (int g = strand; g < parts; g += 32) v += __ldg(part + (long long)g * H + e);
+    for (int g = strand; g < parts; g += 32) v += __ldcg(part + (long long)g * H + e);
   }
   s[strand][lane] = v;
   __syncthreads();

@@ -17,11 +17,11 @@ namespace route {
 // The sequence that row t belongs to, -1 for none: of those that begin at or before it the last.
 __device__ __forceinline__ int sequence_of(const int* off, int B, long long t) {
   if (off == nullptr) return 0;
-  if (t < (long long)__ldg(off) || t >= (long long)__ldg(off + B)) return -1;
+  if (t < (long long)*off || t >= (long long)off[B]) return -1;
   int lo = 0, hi = B;                                       // off[lo] <= t < off[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if ((long long)__ldg(off + mid) <= t) lo = mid; else hi = mid;
+    if ((long long)off[mid] <= t) lo = mid; else hi = mid;
   }
   return lo;
 }
@@ -41,10 +41,10 @@ balance_count_kernel(const BalanceParams p, int rows_per) {
     long long end = hi;
     int b = 0;
     if (p.seq_off != nullptr) {
-      if (at >= (long long)__ldg(p.seq_off + p.B)) break;   // (rows outside all sequences are passed over)
-      if (at < (long long)__ldg(p.seq_off)) { at = (long long)__ldg(p.seq_off); continue; }
+      if (at >= (long long)p.seq_off[p.B]) break;   // (rows outside all sequences are passed over)
+      if (at < (long long)*p.seq_off) { at = (long long)*p.seq_off; continue; }
       b = sequence_of(p.seq_off, p.B, at);
-      end = min(end, (long long)__ldg(p.seq_off + b + 1));
+      end = min(end, (long long)p.seq_off[b + 1]);
     }
     for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
     if (threadIdx.x == 0) s_rows = 0;
@@ -52,7 +52,7 @@ balance_count_kernel(const BalanceParams p, int rows_per) {
     int live = 0;
     for (long long t0 = at + warp * rows_at_once; t0 < end; t0 += (long long)(blockDim.x >> 5) * rows_at_once) {
       const long long t = t0 + sub;
-      const long long i = sub < rows_at_once && t < end ? __ldg(p.idx + t * K + choice) : -1;
+      const long long i = sub < rows_at_once && t < end ? p.idx[t * K + choice] : -1;
       const bool ok = i >= 0 && i < E;
       if (ok) atomicAdd(s_count + (int)i, 1);
       const uint32_t some = __ballot_sync(0xffffffffu, ok);

@@ -114,7 +114,7 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, const L* row, c
       const int e = i * 32 + lane;
       const bool absent = v[i] == -INFINITY;
       v[i] = soft ? exp(v[i] - top) / total : 1.0 / (1.0 + exp(-v[i]));
-      if (p.bias != nullptr && e < E) v[i] += (V)__ldg(p.bias + e);
+      if (p.bias != nullptr && e < E) v[i] += (V)p.bias[e];
       if (absent) v[i] = -INFINITY;
     }
   } else {
@@ -254,7 +254,7 @@ struct Defined {
     if constexpr (computed(MODE)) {
       if (v == (V)-INFINITY) return v;
       v = MODE == kSoftmax ? exp(v - top) / total : 1.0 / (1.0 + exp(-v));
-      if (p.bias != nullptr) v += (V)__ldg(p.bias + e);
+      if (p.bias != nullptr) v += (V)p.bias[e];
     }
     return v;
   }
@@ -330,20 +330,20 @@ __device__ __forceinline__ uint32_t order16(float v, const float*) { return 0u; 
 template <typename L> struct Four;           // four logits in one load
 template <> struct Four<float> {
   static __device__ __forceinline__ void get(const float* p, float* f) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+    const float4 v = *reinterpret_cast<const float4*>(p);
     f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
   }
 };
 template <> struct Four<__nv_bfloat16> {
   static __device__ __forceinline__ void get(const __nv_bfloat16* p, float* f) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
     f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
   }
 };
 template <> struct Four<__half> {
   static __device__ __forceinline__ void get(const __half* p, float* f) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
     f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
   }
@@ -362,7 +362,7 @@ struct Share {
     most_bias = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      bias[i] = computed && p.bias != nullptr && i < n ? __ldg(p.bias + e0 + i) : 0.f;
+      bias[i] = computed && p.bias != nullptr && i < n ? p.bias[e0 + i] : 0.f;
       if (fabsf(bias[i]) < INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
     }
     if (computed) most_bias = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_bias)));

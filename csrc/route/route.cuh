@@ -8,9 +8,11 @@
 namespace b200ep {
 namespace route {
 
-__device__ __forceinline__ float logit(const float* p) { return __ldg(p); }
-__device__ __forceinline__ float logit(const __nv_bfloat16* p) { return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16); }
-__device__ __forceinline__ float logit(const __half* p) { return __half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short*>(p)))); }
+// (coherent loads, here and of all other inputs: the kernel before, in stream order, may still write what this one reads when
+// its CTAs are placed, so the data is not read-only for their lifetime, as the non-coherent path requires)
+__device__ __forceinline__ float logit(const float* p) { return *p; }
+__device__ __forceinline__ float logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float logit(const __half* p) { return __half2float(*p); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }

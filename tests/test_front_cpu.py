@@ -41,6 +41,16 @@ def test_tracing_is_refused(device):
             assert call(x).device == x.device
 
 
+def test_kernels_placed_before_their_inputs_are_complete_read_them_coherently():
+    """Launches in stream order overlap the kernel before: the non-coherent path (and what lets the compiler take it) is for
+    data that nobody writes while the kernel is there, and such loads may be moved in front of the wait."""
+    csrc = Path(__file__).resolve().parent.parent / "csrc"
+    for part in ("norm", "route"):
+        for f in sorted(csrc.glob(f"{part}/*.cu*")):
+            for n, line in enumerate(f.read_text().splitlines(), 1):
+                assert not any(s in line for s in ("__ldg(", "ld_global_nc", "ld.global.nc", "__restrict__")), f"{f.name}:{n}"
+
+
 def test_unknown_scores_are_refused():
     from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
     for call in (lambda: route(torch.randn(2, 8), 2, score="relu"), lambda: balance_loss(torch.randn(2, 8), torch.zeros(2, 2, dtype=torch.int64), score="")):
