@@ -546,9 +546,9 @@ __device__ __forceinline__ int choose(const RouteParams& p, const Groups& gr, co
 }
 
 // Weights of a token's choices, lane k's of choice k: e < 0 for none.
-template <typename L>
+template <typename L, int MODE>
 __device__ __forceinline__ void store_choice(const RouteParams& p, const L* row, long long t, int k, int e, float top, float sum) {
-  const bool soft = p.score == SCORE_SOFTMAX;
+  const bool soft = MODE == kSoftmax || (!computed(MODE) && p.score == SCORE_SOFTMAX);
   float l = 0.f, s = 0.f;
   if (e >= 0) {
     l = logit(row + e);
@@ -563,7 +563,7 @@ __device__ __forceinline__ void store_choice(const RouteParams& p, const L* row,
     if (p.aux != nullptr && !soft) p.aux[t * p.K + k] = l;
   }
   if (p.aux != nullptr && soft && k < 3)
-    p.aux[t * 3 + k] = k == 0 ? top : k == 1 ? (sum > 0.f || sum != sum ? 1.f / sum : 0.f) : kSumEps * reciprocal(chosen + kSumEps);
+    p.aux[t * 3 + k] = k == 0 ? top : k == 1 ? (sum == 0.f ? 0.f : reciprocal(sum)) : kSumEps * reciprocal(chosen + kSumEps);
 }
 
 template <typename L, int VPL, int MODE>
@@ -577,7 +577,7 @@ route_kernel(const __grid_constant__ RouteParams p, const __grid_constant__ Grou
     float top = 0.f, sum = 0.f;
     int e = choose<L, VPL, MODE>(p, gr, mine, row, top, sum);
     if (lane >= p.K) e = -1;
-    store_choice<L>(p, row, t, lane, e, top, sum);
+    store_choice<L, MODE>(p, row, t, lane, e, top, sum);
   }
 }
 
