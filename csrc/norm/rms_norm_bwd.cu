@@ -1,12 +1,13 @@
 // Gradients of the root-mean-square norm with the residual's addition (y = h r w, h = x + residual, r from the forward):
 //   a = dy w,  n = h r,  dx = dresidual = r (a - n mean(a n)) + dh,  dw = sum over the rows of dy n
-// all in f32, rounded where they are stored. Bound: memory (three or four tensors read, one written). h is read as the
-// forward stored it, which costs dw a relative error of one rounding of h (2^-9 for bf16, about that of storing dw in bf16);
-// for weights in f32 the caller passes x and the residual instead and h is summed again: a tensor more, dw exact to 32 bits.
+// all in f32, rounded where they are stored. Bound: memory (three to five tensors read, one written). Of 16-bit rows with a
+// residual h was rounded when the forward stored it. Where dw is wanted the caller passes x and the residual instead and h is
+// summed again, a tensor more: from the stored h, dw had a second rounding's error (bf16 2.33e-3 for 1.64e-3 of its norm; dx, where h
+// stands in a correction alone, 1.6574e-3 for the same, so without dw h is read: 16384 x 7168 158 for 192 us).
 // Persistent CTAs have the next rows under way in shared memory while they are at one (every thread copies what it will need
 // itself), and keep the weights and their part of dw in registers, so that dw costs one row of f32 a CTA, summed in a fixed
-// order by a second launch: the same bits from run to run. One B200, bf16 with a residual: 16384 x 7168 199 us with f32 weights
-// (5.9 TB/s, 91 % of a copy's rate), 166 with bf16 weights, 4095 x 4096 33.5, and 3 to 4 us for the second launch.
+// order by a second launch: the same bits from run to run. One B200, bf16 with a residual: 16384 x 7168 188 to 201 us with f32 weights
+// (5.9 TB/s, 91 % of a copy's rate), 192 with bf16 weights, 4095 x 4096 35.6, and 3 to 4 us for the second launch.
 #include "norm.cuh"
 
 namespace b200ep {

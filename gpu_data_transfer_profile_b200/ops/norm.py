@@ -22,7 +22,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.
              eps: float = 1e-6) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """y, or (y, h) with a residual (shape and type of x): h is the residual of the next block.
 
-    Differentiable once in x, residual and weight; the weight's gradient is summed in a fixed order. No forward-mode
+    Differentiable once in x, residual and weight. Gradients are computed in f32 and rounded once; the weight's is summed in a
+    fixed order. Of 16-bit rows with a residual the backward reads x and residual again where the weight needs a gradient,
+    and keeps both until then; else it reads h as it was stored, a rounding of h in the second term of x's gradient. No forward-mode
     derivatives, no function transforms, no tracing (refused)."""
     y, h = _ext.load().rms_norm(x, weight, residual, eps)
     return y if residual is None else (y, h)

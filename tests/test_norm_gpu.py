@@ -142,6 +142,30 @@ def test_gradients(H, dt, wdt):
         assert got[1].dtype == wdt and ((got[1].double() - ref[1]).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dt,wdt", [(BF16, BF16), (F16, F16), (BF16, F16)])
+@pytest.mark.parametrize("T,H", [(1, 256), (700, 512), (4096, 1024), (333, 1407), (900, 7168), (5, 32768)])
+def test_gradients_of_16_bit_weights_are_rounded_once(T, H, dt, wdt):
+    """With a residual: x and residual, not their stored sum, are what was normalised."""
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm
+    x, r, w = _inputs((T, H), dt, wdt, True, seed=H)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    dy, dh = (torch.randn(T, H, generator=g, device="cuda").to(dt) for _ in range(2))
+    leaves = [t.requires_grad_(True) for t in (x, w, r)]
+    wide = [t.detach().double().requires_grad_(True) for t in leaves]
+    got = torch.autograd.grad(rms_norm(x, w, residual=r, eps=1e-5), leaves, (dy, dh))
+    yw, hw = _wide(*wide, 1e-5)
+    ref = torch.autograd.grad((yw, hw), wide, (dy.double(), dh.double()))
+    h = hw.detach()
+    rstd = torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-5)
+    a, n = dy.double() * w.detach().double(), h * rstd
+    size = rstd * (a.abs() + n.abs() * (a * n).abs().mean(-1, keepdim=True)) + dh.double().abs()
+    tiny = 2.0 ** -25 if F16 in (dt, wdt) else 0
+    assert ((got[0].double() - ref[0]).abs() <= ref[0].abs() * _half(dt) * 1.01 + size * 90 * U_F32 + tiny).all()
+    # T products, each of four roundings in 32 bits, summed T / 148 in a thread, by 8 warps and in up to 600 parts in 8 strands
+    terms = (dy.double() * n).abs().sum(0)
+    assert ((got[1].double() - ref[1]).abs() <= ref[1].abs() * _half(wdt) * 1.01 + terms * (100 + math.ceil(T / 148)) * U_F32 + tiny).all()
+
+
 def test_gradient_against_differences():
     """Directional differences of the forward in 32 bits: d/ds f(x + s u) = <grad, u>."""
     from gpu_data_transfer_profile_b200.ops.norm import rms_norm
