@@ -304,8 +304,8 @@ int launch_balance(const BalanceParams& p, cudaStream_t st) {
   if (!route::fits(p)) return 1;
   if (p.T == 0) return cudaMemsetAsync(p.loss, 0, sizeof(float), st) == cudaSuccess ? 0 : 2;
   if (cudaMemsetAsync(p.counts, 0, (size_t)balance_words(p) * sizeof(int), st) != cudaSuccess) return 2;
-  const int rows_per = (p.T + 295) / 296 < 8 ? 8 : (p.T + 295) / 296;
-  route::balance_count_kernel<<<(p.T + rows_per - 1) / rows_per, 256, 0, st>>>(p, rows_per);
+  const long long share = (p.T + 295LL) / 296, rows_per = share < 8 ? 8 : share;      // (sums in 64 bits: T may be the largest int)
+  route::balance_count_kernel<<<(unsigned)((p.T + rows_per - 1) / rows_per), 256, 0, st>>>(p, (int)rows_per);
   if (p.type == ELEM_BF16) return route::forward<__nv_bfloat16>(p, st);
   if (p.type == ELEM_F16) return route::forward<__half>(p, st);
   return route::forward<float>(p, st);

@@ -575,3 +575,16 @@ def test_offsets_beyond_32_bits():
     del g, w
     g = torch.autograd.grad(balance_loss(l, idx, score="sigmoid", seq_off=off), l)[0]
     assert (g[:1000] == 0).all() and g[-400:].float().norm() > 0 and g[-401].abs().max() == 0
+
+
+def test_balance_loss_of_the_most_rows():
+    """As many rows as an int counts, one expert: every share is 1 and so is the loss."""
+    from gpu_data_transfer_profile_b200.ops.router import balance_loss
+    T = (1 << 31) - 1
+    l = torch.zeros(T, 1, dtype=F16, device="cuda", requires_grad=True)
+    idx = torch.zeros(T, 1, dtype=torch.int64, device="cuda")
+    loss = balance_loss(l, idx)
+    # 1 / T in 32 bits, a share and a count over T likewise: a rounding each, their products one more; the sum is in 64 bits
+    assert abs(loss.item() - 1) <= 6 * U
+    d, = torch.autograd.grad(loss, l)
+    assert d.shape == l.shape and d[::4099].abs().max() == 0 and d[-5:].abs().max() == 0
