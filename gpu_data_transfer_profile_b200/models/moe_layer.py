@@ -133,6 +133,14 @@ class MoELayer(torch.nn.Module):
         # (a loss that hangs on a graph can neither be copied nor stored)
         return {**self.__dict__, "aux_loss": None}
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "norm_weight" not in self._parameters:           # a layer that was stored before it had these options
+            self._choice = dict(score="softmax", num_groups=1, topk_groups=None, group_best=1, renormalize=True, scale=1.0)
+            self._balance, self._plain_choice, self.norm_eps, self.aux_loss = None, True, 1e-6, None
+            self.register_buffer("expert_bias", None)
+            self.register_parameter("norm_weight", None)
+
     def _fused_logits(self, x) -> bool:
         """Whether the router's own kernel may stand in for its product with these rows."""
         return (type(x) is torch.Tensor and x.dtype == torch.bfloat16 and x.dim() == 2 and x.is_contiguous()

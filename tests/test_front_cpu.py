@@ -51,6 +51,24 @@ def test_kernels_placed_before_their_inputs_are_complete_read_them_coherently():
                 assert not any(s in line for s in ("__ldg(", "ld_global_nc", "ld.global.nc", "__restrict__")), f"{f.name}:{n}"
 
 
+def test_layer_stored_before_it_had_a_norm_and_a_choice_of_routers():
+    """Whole modules that earlier versions pickled: the same attributes but those that came with the options."""
+    from gpu_data_transfer_profile_b200.models.moe_layer import MoELayer
+    layer = MoELayer(64, 64, 4, 2, None, dtype=torch.float32, device="cpu", expert_backend="torch")
+    state = layer.__getstate__()
+    new = ("_choice", "_balance", "_plain_choice", "norm_eps", "aux_loss")
+    old = {k: dict(v) if k in ("_buffers", "_parameters") else v for k, v in state.items() if k not in new}
+    del old["_buffers"]["expert_bias"], old["_parameters"]["norm_weight"]
+    again = MoELayer.__new__(MoELayer)
+    again.__setstate__(old)
+    assert sorted(again.state_dict()) == sorted(layer.state_dict()) and all(getattr(again, n) == getattr(layer, n) for n in new)
+    x = torch.randn(5, 64)
+    for a, b in zip(again._route(x, None, True), layer._route(x, None, True)):
+        assert torch.equal(a, b)
+    again._mix = lambda *a: a[0]
+    assert again(x) is x and again.aux_loss is None
+
+
 def test_unknown_scores_are_refused():
     from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
     for call in (lambda: route(torch.randn(2, 8), 2, score="relu"), lambda: balance_loss(torch.randn(2, 8), torch.zeros(2, 2, dtype=torch.int64), score="")):
