@@ -106,6 +106,10 @@ class MoELayer(torch.nn.Module):
             raise ValueError(f"unsupported score {score!r}; expected one of {R.SCORES}")
         if z_coeff and score != "softmax":
             raise ValueError("z_coeff goes with softmax scores")
+        if topk_groups is not None and not 1 <= topk_groups <= num_groups:
+            raise ValueError("topk_groups has to be between 1 and num_groups")
+        if group_best not in (1, 2):
+            raise ValueError("group_best is 1 or 2")
         self._choice = dict(score=score, num_groups=num_groups, topk_groups=topk_groups, group_best=group_best,
                             renormalize=renormalize, scale=route_scale)
         self._balance = dict(score=score, coeff=balance_coeff, z_coeff=z_coeff) if balance_coeff or z_coeff else None

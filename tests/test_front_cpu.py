@@ -69,6 +69,15 @@ def test_layer_stored_before_it_had_a_norm_and_a_choice_of_routers():
     assert again(x) is x and again.aux_loss is None
 
 
+@pytest.mark.parametrize("kw", [dict(topk_groups=2), dict(topk_groups=0), dict(num_groups=2, topk_groups=3), dict(group_best=0), dict(group_best=3)])
+def test_layer_refuses_groups_that_it_could_not_choose(kw):
+    from gpu_data_transfer_profile_b200.models.moe_layer import MoELayer
+    with pytest.raises(ValueError, match="group"):
+        MoELayer(64, 64, 4, 2, None, dtype=torch.float32, device="cpu", expert_backend="torch", **kw)
+    for good in (dict(topk_groups=1), dict(group_best=2), dict(num_groups=2, topk_groups=2)):
+        MoELayer(64, 64, 4, 2, None, dtype=torch.float32, device="cpu", expert_backend="torch", **good)
+
+
 def test_unknown_scores_are_refused():
     from gpu_data_transfer_profile_b200.ops.router import balance_loss, route
     for call in (lambda: route(torch.randn(2, 8), 2, score="relu"), lambda: balance_loss(torch.randn(2, 8), torch.zeros(2, 2, dtype=torch.int64), score="")):
