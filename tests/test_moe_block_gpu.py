@@ -187,6 +187,25 @@ def test_fp8_rows_of_the_norm_go_straight_into_the_exchange(world, T, monkeypatc
     assert (err < 0.12).float().mean() >= 0.97
 
 
+@pytest.mark.parametrize("T", [1, 37, 200])
+@pytest.mark.parametrize("residual", [False, True])
+def test_fp8_rows_of_the_norm_with_the_default_choice(world, T, residual, monkeypatch):
+    """Without options that may leave a choice out, a group of one takes the rows in place without the receive count."""
+    from gpu_data_transfer_profile_b200.parallel.buffer import Buffer
+    layer = _layer(world, use_fp8=True, norm=True)
+    x, r = (torch.randn(T, 256, device="cuda").to(torch.bfloat16) for _ in range(2))
+    seen = []
+    real = Buffer._dispatch_own_probs
+    monkeypatch.setattr(Buffer, "_dispatch_own_probs", lambda self, rows, *a: seen.append([t.dtype for t in rows]) or real(self, rows, *a))
+    with torch.no_grad():
+        out, h = layer(x, residual=r if residual else None)
+    assert seen == [[torch.float8_e4m3fn, torch.float32]]
+    assert torch.equal(h, (x.float() + r.float()).to(torch.bfloat16) if residual else x)
+    ref, _, _, _ = _reference(layer, x, None, r if residual else None, None)
+    err = (out.float() - ref).norm(dim=1) / ref.norm(dim=1)
+    assert (err < 0.12).float().mean() >= 0.97                     # (as above)
+
+
 def test_router_logits_kernel_against_64_bits():
     from gpu_data_transfer_profile_b200 import _ext
     C = _ext.load()

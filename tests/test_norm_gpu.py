@@ -330,6 +330,33 @@ def test_fp8_rows_feed_the_grouped_gemm():
     assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + size * 2.0 ** -13).all()
 
 
+def test_widths_in_turn_and_two_threads():
+    """One kernel serves several widths, with and without a residual: every call is launched by its own sizes."""
+    import threading
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm
+    calls = []
+    for H, residual in ((7168, True), (1536, True), (7168, False), (4096, True), (1536, False)):
+        x, r, w = _inputs((611, H), BF16, BF16, residual, seed=H)
+        calls.append((x, r, w, rms_norm(x, w, residual=r)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(order):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for k in range(60):
+                x, r, w, want = calls[(k * order) % len(calls)]
+                got = rms_norm(x, w, residual=r)
+                same = torch.equal(got, want) if r is None else torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+                if not same:
+                    bad.append((k, x.shape, r is None))
+    threads = [threading.Thread(target=work, args=(o,)) for o in (1, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_refusals():
     from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
     x, r, w = _inputs((6, 256), BF16, BF16, True)
