@@ -11,6 +11,8 @@ namespace b200ep {
 namespace norm {
 
 template <typename T> constexpr int kEpv = 16 / (int)sizeof(T);      // elements of a vector
+// vectors that the longest row lies in
+template <typename T, bool ALIGNED> constexpr int kMaxVecs = kNormMaxHidden / kEpv<T> + (ALIGNED ? 0 : 1);
 
 template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
@@ -153,8 +155,8 @@ __device__ __forceinline__ void fetch_wait(int left) {
   else asm volatile("cp.async.wait_group 3;" ::: "memory");
 }
 constexpr int kMaxStages = 4;            // rows that a thread has under way, for fetch_wait
-// Rows come by way of shared memory unless they are so long (more than 2048 vectors) that their tensors do not fit there:
-// those are loads enough at a time by themselves.
+// Rows come by way of shared memory unless they are so long (more than 2048 vectors of 16-bit elements, 4096 of f32) that their
+// tensors do not fit there: those are loads enough at a time by themselves.
 template <typename T, int VPT, bool WARP> constexpr bool kStaged = WARP || VPT * kEpv<T> <= 16;
 
 // The weights of one vector of rows in T, kept as they are stored (W: T or float) so that they take few registers.

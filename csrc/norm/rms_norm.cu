@@ -163,10 +163,14 @@ int launch_fwd_sized(const NormFwdParams& p, cudaStream_t st) {
   // The cast of 16-bit rows wants more warps (8191 x 7168: 95.7 us with two vectors a thread, 90.2 with one), without it, and
   // of f32 rows, fewer and longer threads are as good or better (12001 x 1408 in f16: 14.6 and 16.7; 8191 x 4096 in f32 to
   // fp8: 52.0 and 68.8).
-  if (FP8 && sizeof(T) == 2 && nvec > 256 && nvec <= 1024) return launch_fwd<T, W, 1, FP8, false, ALIGNED>(p, threads(1), st);
+  if constexpr (FP8 && sizeof(T) == 2) {
+    if (nvec > 256 && nvec <= 1024) return launch_fwd<T, W, 1, FP8, false, ALIGNED>(p, threads(1), st);
+  }
   if (nvec <= 2048) return launch_fwd<T, W, 2, FP8, false, ALIGNED>(p, threads(2), st);
-  if (nvec <= 4096) return launch_fwd<T, W, 4, FP8, false, ALIGNED>(p, threads(4), st);
-  return launch_fwd<T, W, 9, FP8, false, ALIGNED>(p, threads(9), st);
+  if constexpr (kMaxVecs<T, ALIGNED> > 4096) {
+    if (nvec > 4096) return launch_fwd<T, W, 9, FP8, false, ALIGNED>(p, threads(9), st);
+  }
+  return launch_fwd<T, W, 4, FP8, false, ALIGNED>(p, threads(4), st);
 }
 
 template <typename T, typename W>

@@ -228,8 +228,10 @@ int bwd_sized(const NormBwdParams& p, int* parts, cudaStream_t st) {
   // 198; 16384 x 4096 with 512 102 us, with 256 98.5; 4096 x 8192 in f32 with 1024 83 us, with 512 66
   if (nvec <= 256) return run_bwd<T, W, 1, false, ALIGNED>(p, threads(1), parts, st);
   if (nvec <= (sizeof(T) == 4 ? 1024 : 2048)) return run_bwd<T, W, 2, false, ALIGNED>(p, threads(2), parts, st);
-  if (nvec <= 4096) return run_bwd<T, W, 4, false, ALIGNED>(p, threads(4), parts, st);
-  return run_bwd<T, W, 9, false, ALIGNED>(p, threads(9), parts, st);
+  if constexpr (kMaxVecs<T, ALIGNED> > 4096) {
+    if (nvec > 4096) return run_bwd<T, W, 9, false, ALIGNED>(p, threads(9), parts, st);
+  }
+  return run_bwd<T, W, 4, false, ALIGNED>(p, threads(4), parts, st);
 }
 
 template <typename T, typename W>

@@ -325,7 +325,6 @@ __device__ __forceinline__ uint32_t order16(float v, const __half*) {
   const uint32_t u = (uint32_t)__half_as_ushort(__float2half_rn(v)) << 16;
   return (u ^ ((uint32_t)((int)u >> 31) | 0x80000000u)) & 0xffff0000u;
 }
-__device__ __forceinline__ uint32_t order16(float v, const float*) { return 0u; }      // (has no such mode)
 
 template <typename L> struct Four;           // four logits in one load
 template <> struct Four<float> {
@@ -440,12 +439,6 @@ __device__ __forceinline__ int choose(const RouteParams& p, const Groups& gr, co
       }
     }
   }
-  // whether two values, the first with the higher key, are in this order for certain
-  const auto apart = [&](uint32_t high, uint32_t low) {
-    if (MODE == kLogit16 || low <= kAbsent) return true;
-    if (MODE == kLogit32) return (high & ~MASK) > (low & ~MASK) && !(low >= (0x7fffffffu & ~MASK) && high <= (0x80000000u | MASK));      // (-0 is 0)
-    return Key32::value(high) - Key32::value(low) > 2.f * margin;
-  };
   sort_keys(key);
   bool exact = gr.exact || (!computed(MODE) && __any_sync(0xffffffffu, odd));
   if (gr.count > 1) {
@@ -522,6 +515,12 @@ __device__ __forceinline__ int choose(const RouteParams& p, const Groups& gr, co
   uint2 pick = picks[lane];
   int e = lane < n ? (int)pick.y : -1;
   if constexpr (MODE != kLogit16) {
+    // whether two values, the first with the higher key, are in this order for certain
+    const auto apart = [&](uint32_t high, uint32_t low) {
+      if (low <= kAbsent) return true;
+      if (MODE == kLogit32) return (high & ~MASK) > (low & ~MASK) && !(low >= (0x7fffffffu & ~MASK) && high <= (0x80000000u | MASK));      // (-0 is 0)
+      return Key32::value(high) - Key32::value(low) > 2.f * margin;
+    };
     uint32_t next = n == p.K ? __reduce_max_sync(0xffffffffu, key[0]) : 0u;
     const uint32_t follows = __shfl_down_sync(0xffffffffu, pick.x, 1), after = lane + 1 < n ? follows : next;
     const bool doubt = lane < n && !apart(pick.x, after);

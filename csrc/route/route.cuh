@@ -1,4 +1,5 @@
-// What the choice of experts and the balance loss share: a warp has a token, lane l the experts l, l + 32, ...
+// What the choice of experts and the balance loss share. A warp has a token. In the balance loss, and where the choice is made
+// exactly as it is defined, lane l has the experts l, l + 32, ...; in the quick way of the choice, a run of neighbours.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
