@@ -255,9 +255,13 @@ balance_bwd_kernel(const BalanceBwdParams a, int rows_per_warp) {
   }
 }
 
+// Multiprocessors of a B200. How the rows are split is a matter of speed alone, has to be the same where room is made for the parts
+// and where they are written, and is worked out several times in calls that are bound by host time: not asked of the runtime.
+constexpr long long kSms = 148;
+
 inline int rows_a_warp(int T) {
-  // four CTAs of 8 warps on each of 148 SMs, each warp a run of neighbouring rows
-  const long long warps = 148LL * 4 * kBalanceWarps;
+  // four CTAs of 8 warps on every SM, each warp a run of neighbouring rows
+  const long long warps = kSms * 4 * kBalanceWarps;
   return (int)((T + warps - 1) / warps) < 1 ? 1 : (int)((T + warps - 1) / warps);
 }
 inline int ctas(int T) {
@@ -304,7 +308,7 @@ int launch_balance(const BalanceParams& p, cudaStream_t st) {
   if (!route::fits(p)) return 1;
   if (p.T == 0) return cudaMemsetAsync(p.loss, 0, sizeof(float), st) == cudaSuccess ? 0 : 2;
   if (cudaMemsetAsync(p.counts, 0, (size_t)balance_words(p) * sizeof(int), st) != cudaSuccess) return 2;
-  const long long share = (p.T + 295LL) / 296, rows_per = share < 8 ? 8 : share;      // (sums in 64 bits: T may be the largest int)
+  const long long ctas = 2 * route::kSms, share = (p.T + ctas - 1) / ctas, rows_per = share < 8 ? 8 : share;      // (64 bits: T may be the largest int)
   route::balance_count_kernel<<<(unsigned)((p.T + rows_per - 1) / rows_per), 256, 0, st>>>(p, (int)rows_per);
   if (p.type == ELEM_BF16) return route::forward<__nv_bfloat16>(p, st);
   if (p.type == ELEM_F16) return route::forward<__half>(p, st);

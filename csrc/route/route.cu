@@ -210,7 +210,8 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
 }
 
 // 1 / y, off by little more than half a unit in the last place: the hardware's approximation and one step of Newton's
-// iteration; without the branches of a division.
+// iteration; without the branches of a division. It has no denormals: 0 for y above 2^126, that is for a sigmoid of a logit
+// below -87.3, which is less than the smallest normal number (1.2e-38).
 __device__ __forceinline__ float reciprocal(float y) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
@@ -424,6 +425,8 @@ __device__ __forceinline__ int choose(const RouteParams& p, const Groups& gr, co
     }
   } else {
     if (soft) {
+      // (the approximate exponential is off by 2 + 1.2 d units in the last place at a distance d to the maximum, where a term is e^-d:
+      // the sum of up to 1024, and so every weight that is not renormalised, by less than 8 units, 2^-20 of itself)
 #pragma unroll
       for (int i = 0; i < VPL; ++i) sum += __expf(l[i] - top);
       sum = warp_sum(sum);
@@ -648,6 +651,10 @@ route_bwd_kernel(const RouteBwdParams p) {
 
 template <typename L, int VPL, int MODE>
 int launch_sized(const RouteParams& p, const Groups& g, cudaStream_t st) {
+  // Fewer tokens than 8 for each of 148 SMs: a CTA of its own for each, so that one that is settled or compared exactly keeps no
+  // other's SM busy. us with one warp a CTA and with eight: 256 sigmoid scores with a bias in 8 groups 3.61 and 4.04 for 300
+  // tokens, 5.02 and 4.98 for 1183, 7.45 and 7.99 for 4096; 64 softmax scores by their logits, where little is ever looked at
+  // again, 2.94 and 2.88, 3.24 and 2.96, 4.95 and 3.92.
   const int warps = p.T < 1184 ? 1 : 8;
   const auto kern = route_kernel<L, VPL, MODE>;
   static std::atomic<int> fits[2];                          // CTAs per SM with 1 and with 8 warps; 0: not asked yet
@@ -680,6 +687,7 @@ Groups lay_groups(const RouteParams& p, bool told_apart) {
 template <typename L, int MODE>
 int launch_mode(const RouteParams& p, cudaStream_t st) {
   Groups g = lay_groups<L>(p, true);
+  // (4096 x 1020 in 17 groups 245 us, 4096 x 1024 in 16 groups, which have a quick way, 44)
   if (g.chunk > 32) {
     g = lay_groups<L>(p, false);
     g.exact = true;
