@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kSendWarps * 32, 2)
 dispatch_send_kernel(EpGeom g, EpRegions rg, const __grid_constant__ PeerPtrs peers, EpMeta m,
                      const char* __restrict__ x, int row_bytes_in, int parts,
                      const long long* __restrict__ topk_idx, const float* __restrict__ topk_w,
-                     const int* __restrict__ item_rank, const int* __restrict__ chunk_base,
+                     const int* item_rank, const int* chunk_base,
                      int* send_row, int* send_slot, unsigned int* block_counter, int* host_word,
                      int* status, const float* __restrict__ scales_in) {
   stream_order_wait();

@@ -153,7 +153,7 @@ constexpr int kNotifyWarps = 8;
 // shared memory (expert mode only), `hist` the chunk's row of B counts (shared or global memory).
 template <int MODE>
 __device__ __forceinline__ void notify_chunk(const EpGeom& g, int c, int lane, unsigned int* bits,
-                                             const bool* __restrict__ is_in_rank,
+                                             const bool* is_in_rank,
                                              const long long* __restrict__ topk_idx,
                                              int* __restrict__ item_rank, int* hist, int* status) {
   const int J = g.J, B = g.B, R = g.R, E = g.E, K = g.K;
@@ -218,7 +218,7 @@ __device__ __forceinline__ void notify_chunk(const EpGeom& g, int c, int lane, u
 // before the flag for every observer (release cumulativity).
 template <int MODE>
 __device__ __forceinline__ void notify_publish(const EpGeom& g, const EpRegions& rg, const PeerPtrs& peers,
-                                               const int* __restrict__ num_tokens_per_expert,
+                                               const int* num_tokens_per_expert,
                                                const int* hist, int* vec) {
   const int R = g.R, E = g.E, V = R + E;
   if (MODE == 0) {
@@ -302,9 +302,9 @@ __device__ __forceinline__ void notify_scan(int* chunk_hist, int* hist, int B, i
 
 template <int MODE>
 __global__ void __launch_bounds__(kNotifyWarps * 32)
-notify_send_kernel(EpGeom g, EpRegions rg, const __grid_constant__ PeerPtrs peers, const bool* __restrict__ is_in_rank,
+notify_send_kernel(EpGeom g, EpRegions rg, const __grid_constant__ PeerPtrs peers, const bool* is_in_rank,
                    const long long* __restrict__ topk_idx,
-                   const int* __restrict__ num_tokens_per_expert, int* __restrict__ item_rank,
+                   const int* num_tokens_per_expert, int* __restrict__ item_rank,
                    int* chunk_hist, unsigned int* block_counter, int* status) {
   extern __shared__ int sh[];
   stream_order_wait();
@@ -330,9 +330,9 @@ notify_send_kernel(EpGeom g, EpRegions rg, const __grid_constant__ PeerPtrs peer
 template <int MODE>
 __global__ void __cluster_dims__(kSmallCluster, 1, 1) __launch_bounds__(kSmallClusterThreads, 1)
 notify_send_cluster_kernel(EpGeom g, EpRegions rg, const __grid_constant__ PeerPtrs peers,
-                           const bool* __restrict__ is_in_rank,
+                           const bool* is_in_rank,
                            const long long* __restrict__ topk_idx,
-                           const int* __restrict__ num_tokens_per_expert,
+                           const int* num_tokens_per_expert,
                            int* __restrict__ item_rank, int* chunk_base, int per, int* status) {
   extern __shared__ int sh[];
   constexpr int kWarps = kSmallClusterThreads / 32;

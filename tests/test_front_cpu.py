@@ -1,5 +1,6 @@
 """Norm, routing and balance loss without a GPU: what is refused before anything is launched, and their cases."""
 import random
+import re
 import sys
 from pathlib import Path
 
@@ -49,6 +50,9 @@ def test_kernels_placed_before_their_inputs_are_complete_read_them_coherently():
         for f in sorted(csrc.glob(f"{part}/*.cu*")):
             for n, line in enumerate(f.read_text().splitlines(), 1):
                 assert not any(s in line for s in ("__ldg(", "ld_global_nc", "ld.global.nc", "__restrict__")), f"{f.name}:{n}"
+    # in an exchange: the layout's results in the counts, the counts' results in the dispatch
+    for f in ("layout", "dispatch"):
+        assert not re.search(r"const \w+\* __restrict__ (is_in_rank|num_tokens_per_expert|item_rank|chunk_base)\b", (csrc / "ep" / f"{f}.cu").read_text())
 
 
 def test_layer_stored_before_it_had_a_norm_and_a_choice_of_routers():
