@@ -7,7 +7,8 @@
 // Persistent CTAs have the next rows under way in shared memory while they are at one (every thread copies what it will need
 // itself), and keep the weights and their part of dw in registers, so that dw costs one row of f32 a CTA, summed in a fixed
 // order by a second launch: the same bits from run to run. One B200, bf16 with a residual: 16384 x 7168 188 to 201 us with f32 weights
-// (5.9 TB/s or more, 91 % of a copy's rate), 192 with bf16 weights, 4095 x 4096 35.5 to 38.7, and 3 to 4 us for the second launch.
+// (5.9 TB/s or more, 91 % of a copy's rate), 192 with bf16 weights, 4095 x 4096 35.5 to 38.7, and 3 to 4 us for the second
+// launch. The two-vector form spills 32 to 40 bytes a thread.
 #include "norm.cuh"
 
 namespace b200ep {

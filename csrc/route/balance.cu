@@ -7,8 +7,9 @@
 // With the counts known the loss is a sum over tokens of F_t, so that the logits are read once forward and once backward:
 // a launch that counts the choices (whole numbers: any order gives the same), one that sums F_t (in 64 bits, in a fixed
 // order). A warp has a run of neighbouring rows and keeps f of their sequence in registers. Bound: latency, of launches for
-// few tokens and of the reductions over a row for many: 16384 x 64 in softmax take 3.0 + 8.9 us forward and 8.2 backward on
-// one B200, where the logits' bytes would take 0.6 each time.
+// few tokens and of the reductions over a row for many: 16384 x 64 in softmax take 2.9 + 8.8 us forward and 8.2 backward on
+// one B200, where the logits' bytes would take 0.6 each time; 8191 x 256 in sigmoid 2.7 + 9.8 and 13.2, where the backward's eight
+// counts of 64 bits a lane spill 92 bytes a thread.
 #include "route.cuh"
 
 namespace b200ep {

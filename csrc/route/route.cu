@@ -8,9 +8,10 @@
 // so close that 32 bits choose another expert for one token in some ten thousand. Where v ranks as the logits do, their own
 // 32 bits are compared. Not a number ranks above everything, as in torch.topk.
 // A warp has a token: its lanes hold runs of neighbouring experts of one group, so that a group's best are found inside a
-// lane and a few shuffles. Bound: instructions, about 780 a token of 256 experts in 8 groups (16383 of them, top-8, sigmoid
-// with a bias: 18.3 us on one B200, 70 % of the issue slots; every value in 64 bits: 55.5), for few tokens latency (128: 4.4,
-// or 6.7 with a token that needs 64 bits). The logits are read once.
+// lane and a few shuffles. Bound: instructions, about 790 a token of 256 experts in 8 groups (16383 of them, top-8, sigmoid
+// with a bias: 18.4 to 20.5 us on one B200, 70 % of the issue slots, 76 bytes a thread spilled across the calls of the ways of looking
+// again; every value in 64 bits: 55.5), for few tokens latency (128: 3.6, or 6.7 with a token that needs 64 bits). The logits
+// are read once.
 #include <atomic>
 #include "route.cuh"
 

@@ -88,7 +88,9 @@ class MoELayer(torch.nn.Module):
     `expert_bias=True` adds the buffer `expert_bias` (f32 [E], zeros) that the choice is made with: the program moves it
     towards a balanced load. With `balance_coeff` or `z_coeff`, a forward pass with gradients leaves
     `ops.router.balance_loss` of its (this rank's) choices in `aux_loss`, for the program to add to its loss; without
-    gradients `aux_loss` is None. A choice of -1 (a router logit of -inf) goes to no expert.
+    gradients `aux_loss` is None. With any of these options a choice of -1 (a router logit of -inf) goes to no expert; an inference
+    pass then waits on the host for the number of rows received, also in a group of one (the default choice, which never
+    leaves one out, does not).
     `norm=True` puts `ops.norm.rms_norm` with the parameter `norm_weight` in front: `forward` then takes the residual as
     well and returns (output, hidden_states + residual)."""
 
