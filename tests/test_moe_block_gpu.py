@@ -239,3 +239,54 @@ def test_state_of_a_default_layer_is_what_it_was(world):
     layer = _layer(world)
     assert sorted(layer.state_dict()) == ["experts.weight1", "experts.weight2", "router.weight"]
     assert sorted(_layer(world, norm=True, **GROUPED).state_dict()) == ["expert_bias", "experts.weight1", "experts.weight2", "norm_weight", "router.weight"]
+
+
+@pytest.mark.parametrize("R", [1, 2, 4])
+@pytest.mark.parametrize("fp8", [True, False])
+def test_norm_choice_exchange_over_ranks(R, fp8):
+    """Rows of the norm and ids and weights of the choice, padding among them, through an exchange by expert and back: a
+    token comes back as itself times the sum of its weights, each times what tells its expert."""
+    from gpu_data_transfer_profile_b200.ops.norm import rms_norm, rms_norm_fp8
+    from gpu_data_transfer_profile_b200.ops.router import route
+    from gpu_data_transfer_profile_b200.parallel.local import LocalGroup
+    H, E, K = 512, 16, 4
+    g = LocalGroup(R, 64 << 20, timeout_s=2.0)
+    try:
+        gen = torch.Generator(device="cuda").manual_seed(R)
+        xs, ids, ws, dense = [], [], [], []
+        for r in range(R):
+            T = 60 + 13 * r
+            x, h = (torch.randn(T, H, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2))
+            w = 1 + 0.2 * torch.randn(H, generator=gen, device="cuda")
+            l = torch.randn(T, E, generator=gen, device="cuda")
+            l[T - 7:] = -math.inf
+            l[3, 2:] = -math.inf
+            idx, wt = route(l, K, score="sigmoid", bias=torch.linspace(-0.1, 0.1, E, device="cuda"), num_groups=4, topk_groups=2, group_best=2, scale=2.5)
+            if fp8:
+                (q, s), _, _ = rms_norm_fp8(x, w, residual=h)
+                xs.append((q, s))
+                dense.append((q.double().view(T, H // 128, 128) * s.double()[..., None]).view(T, H))
+            else:
+                xs.append(rms_norm(x, w, residual=h)[0])
+                dense.append(xs[-1].double())
+            ids.append(idx)
+            ws.append(wt)
+        outs = g.dispatch(xs, topk_idx=ids, topk_weights=ws, group_by_expert=True, num_experts=E)
+        ys = []
+        for r, (rows, _, _, counts, handle) in enumerate(outs):
+            el = torch.arange(E // R, device="cuda") + r * (E // R) + 1.0
+            factor = torch.repeat_interleave(el, torch.tensor(counts, device="cuda")) * handle.recv_prob
+            n = factor.numel()
+            assert n == sum(int(((i >= r * (E // R)) & (i < (r + 1) * (E // R))).sum()) for i in ids)
+            got = (rows[0].float().view(-1, H // 128, 128) * rows[1][..., None]).view(-1, H) if fp8 else rows.float()
+            ys.append((got[:n] * factor[:, None]).to(torch.bfloat16))
+        comb = g.combine(ys, [o[4] for o in outs])
+        for r in range(R):
+            gain = (ws[r].double() * (ids[r] + 1) * (ids[r] >= 0)).sum(1, keepdim=True)
+            want = dense[r] * gain
+            # a rounding to bf16 of every row, and one of their sum
+            assert ((comb[r][0].double() - want).abs() <= dense[r].abs() * gain * 2.02 * 2.0 ** -8).all()
+            assert (comb[r][0][-7:] == 0).all()
+        g.check_status()
+    finally:
+        g.destroy()
