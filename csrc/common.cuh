@@ -163,8 +163,9 @@ __device__ __forceinline__ void st_global_v8(void* p, const u32x8& r) {
 // A kernel launched by launch_ordered may be placed on the GPU while the kernel before it on the stream
 // still runs; stream_order_wait, its first statement, holds every thread until that kernel has completed
 // and its writes are visible, so that only launch latency and CTA placement overlap, never the work.
-// Every kernel of a chain waits, so completion is transitive. What the kernel before writes is read by coherent loads (and not by way of
-// a restricted pointer to const, which lets the compiler take others): it is not read-only while this one is there. stream_order_next lets the NEXT kernel be
+// Every kernel of a chain waits, so completion is transitive. What the kernel before writes is read by coherent
+// loads (and not by way of a restricted pointer to const, which lets the compiler take others): it is not
+// read-only while this one is there. stream_order_next lets the NEXT kernel be
 // placed as soon as all CTAs of this one have said so (or ended); a kernel that may wait for peers does
 // not say so: the next one's idle CTAs would keep other streams' kernels from the SMs.
 // Used by the short kernels of an exchange (layout, counts, dispatch, clone, combine: 4096 x 7168 62.6 -> 56.8

@@ -111,8 +111,8 @@ __device__ __forceinline__ void store_vec(char* at, int e0, int H, const uint4& 
   }
 }
 
-// A row's vector straight from memory, zeros outside the row. (Coherent loads, as of all inputs: the kernel before, in stream order,
-// may still write what this one reads when its CTAs are placed.)
+// A row's vector straight from memory, zeros outside the row. (Coherent loads, as of all inputs: the kernel before, in
+// stream order, may still write what this one reads when its CTAs are placed.)
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ uint4 load_vec(const T* row, int e0, int H) {
   if (ALIGNED || whole<T>(e0, H)) return ld_global_once_v4(row + e0);

@@ -24,8 +24,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: Optional[torch.
 
     Differentiable once in x, residual and weight. Gradients are computed in f32 and rounded once; the weight's is summed in a
     fixed order. Of 16-bit rows with a residual the backward reads x and residual again where the weight needs a gradient,
-    and keeps both until then; else it reads h as it was stored, a rounding of h in the second term of x's gradient. No forward-mode
-    derivatives, no function transforms, no tracing (refused)."""
+    and keeps both until then; else it reads h as it was stored, a rounding of h in the second term of x's gradient. No
+    forward-mode derivatives, no function transforms, no tracing (refused)."""
     y, h = _ext.load().rms_norm(x, weight, residual, eps)
     return y if residual is None else (y, h)
 
